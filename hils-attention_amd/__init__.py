@@ -17,3 +17,5 @@ from .ops.hils_fwd_bwd_head import prepare_kv_workspace  # noqa: F401
 from .utils.hils_cache_utils import HiLSDynamicLayer, HiLSPagedLayer, paged_hils_attend  # noqa: F401
 from .ops.rope_tilelang_fp32 import rope_rotary_pos_emb, single_tensor_rope_autograd  # noqa: F401
 from .ops.norm_rope_pool import norm_rope_pool  # noqa: F401
+from .ops.rotary import rotary_embedding, rotary_frequencies  # noqa: F401
+from .ops.paged_cache import copy_pages, paged_accept, paged_append, paged_flex_attn  # noqa: F401

@@ -859,6 +859,275 @@ Tensor chunk_log_z(const Tensor& q, const Tensor& k, int64_t chunk, int64_t wind
   return LogzFn::forward(nullptr, q.contiguous(), kc, chunk, window, scale, mask_lmk);
 }
 
+// ---- rotary positions, and new or drafted tokens on a paged cache ------------------------------
+// The calls below run on the device of their tensors, on that device's current stream.
+void same_device(const char* name, const Tensor& like, std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    if (t->defined() && t->device() != like.device())
+      throw std::runtime_error(c10::str(name, ": tensors on ", like.device().str(), " and ", t->device().str()));
+}
+
+// (B, T, heads, D) rows the kernels can read where they are: contiguous features, everything at multiples of 16 bytes
+Tensor strided_rows(const Tensor& t) {
+  const bool fits = t.stride(3) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 && t.stride(2) % 8 == 0 &&
+                    t.stride(0) >= 0 && t.stride(1) >= 0 && t.stride(2) >= 0 && (uintptr_t)t.const_data_ptr() % 16 == 0;
+  if (fits) return t;
+  const Tensor c = t.contiguous();
+  return (uintptr_t)c.const_data_ptr() % 16 ? c.clone(at::MemoryFormat::Contiguous) : c;
+}
+#define ROW_STRIDES(t) (size_t)(t).stride(0), (size_t)(t).stride(1), (size_t)(t).stride(2)
+
+struct Turn {
+  Tensor positions, inv_freq;
+  int64_t first, interleaved;
+  double scale;
+};
+
+// positions (T) or (B, T) int32 / int64, or none; inv_freq fp32 or fp64
+void check_turn(const char* name, const Turn& c, const Tensor& like, int64_t B, int64_t T, int64_t D, bool per_batch) {
+  HOST_ASSERT(c.inv_freq.defined() && c.inv_freq.dim() == 1 &&
+                  (c.inv_freq.scalar_type() == at::kDouble || c.inv_freq.scalar_type() == at::kFloat) && c.inv_freq.is_contiguous(),
+              name, ": inv_freq must be a contiguous vector, fp32 or fp64");
+  const int64_t R = 2 * c.inv_freq.numel();
+  HOST_ASSERT(R > 0 && R % 16 == 0 && R <= D, name, ": inv_freq of ", c.inv_freq.numel(),
+              " frequencies: twice that must be a multiple of 16 up to the head dim ", D);
+  if (c.inv_freq.requires_grad()) throw std::runtime_error(c10::str(name, ": inv_freq gets no gradient"));
+  HOST_ASSERT(std::isfinite(c.scale), name, ": scale must be finite");
+  same_device(name, like, {&c.inv_freq, &c.positions});
+  if (!c.positions.defined()) return;
+  const at::ScalarType dt = c.positions.scalar_type();
+  if (dt != at::kInt && dt != at::kLong) throw py::type_error(c10::str(name, ": positions must be int32 or int64, got ", c.positions.dtype().name()));
+  HOST_ASSERT((!per_batch && c.positions.sizes() == at::IntArrayRef({T})) || c.positions.sizes() == at::IntArrayRef({B, T}), name,
+              ": positions ", c.positions.sizes(), per_batch ? " must be (B, T) = (" : " must be (T) or (B, T) = (", B, ", ", T, ")");
+}
+
+std::tuple<Tensor, Tensor> rotary_apply(const Tensor& q, const Tensor& k, const Turn& c, double sign);
+
+// One rotation of one or two tensors (either may be missing).
+std::tuple<Tensor, Tensor> rotary_forward(const Tensor& q, const Tensor& k, const Turn& c, double sign) {
+  if (!q.defined()) {
+    if (!k.defined()) return {Tensor(), Tensor()};
+    return {Tensor(), std::get<0>(rotary_forward(k, Tensor(), c, sign))};
+  }
+  const c10::DeviceGuard on(q.device());
+  const int64_t B = q.size(0), T = q.size(1), HQ = q.size(2), D = q.size(3), H = k.defined() ? k.size(2) : 0;
+  Tensor qo = new_tensor({B, T, HQ, D}, q, q.scalar_type());
+  Tensor ko = k.defined() ? new_tensor({B, T, H, D}, k, k.scalar_type()) : Tensor();
+  if (B * T == 0 || HQ == 0 || (k.defined() && H == 0)) {
+    if (HQ == 0 && k.defined() && B * T * H > 0) ko = std::get<0>(rotary_forward(k, Tensor(), c, sign));
+    if (HQ > 0 && B * T > 0) qo = std::get<0>(rotary_forward(q, Tensor(), c, sign));
+    return {qo, ko};
+  }
+  const Tensor qs = strided_rows(q), ks = k.defined() ? strided_rows(k) : Tensor();
+  const Tensor pos = c.positions.defined() ? c.positions.contiguous() : Tensor();
+  HILS_CALL(hils_rotary, cptr(qs), cptr(ks), mptr(qo), mptr(ko), cptr(pos), cptr(c.inv_freq), ROW_STRIDES(qs),
+            (size_t)(H ? ks.stride(0) : 0), (size_t)(H ? ks.stride(1) : 0), (size_t)(H ? ks.stride(2) : 0), i32(B), i32(T),
+            i32(HQ), i32(H), i32(D), i32(2 * c.inv_freq.numel()), i32(c.interleaved),
+            (int)(pos.defined() && pos.scalar_type() == at::kLong), (int)(pos.defined() && pos.dim() == 2), i32(c.first),
+            (int)(c.inv_freq.scalar_type() == at::kDouble), (float)c.scale, (float)sign);
+  return {qo, ko};
+}
+
+struct RotaryFn : torch::autograd::Function<RotaryFn> {
+  static variable_list forward(AutogradContext* ctx, const OptTensor& q, const OptTensor& k, const Turn& c, double sign) {
+    ctx->set_materialize_grads(false);
+    auto [qo, ko] = rotary_forward(opt(q), opt(k), c, sign);
+    ctx->save_for_backward({c.positions, c.inv_freq});
+    ctx->saved_data["cfg"] = std::vector<int64_t>{c.first, c.interleaved, q.has_value(), k.has_value()};
+    ctx->saved_data["scale"] = std::vector<double>{c.scale, sign};
+    variable_list out;  // (a missing tensor is no output)
+    if (q.has_value()) out.push_back(qo);
+    if (k.has_value()) out.push_back(ko);
+    return out;
+  }
+  // the transposed map: the same rotation the other way round
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const auto s = ctx->get_saved_variables();
+    const auto cfg = ctx->saved_data["cfg"].toIntVector();
+    const auto by = ctx->saved_data["scale"].toDoubleVector();
+    auto [dq, dk] = rotary_apply(cfg[2] ? g[0] : Tensor(), cfg[3] ? g.back() : Tensor(),
+                                 Turn{s[0], s[1], cfg[0], cfg[1], by[0]}, -by[1]);
+    return {dq, dk, Tensor(), Tensor()};
+  }
+};
+
+std::tuple<Tensor, Tensor> rotary_apply(const Tensor& q, const Tensor& k, const Turn& c, double sign) {
+  if (!wants_grad({&q, &k})) return rotary_forward(q, k, c, sign);
+  if (!q.defined() && !k.defined()) return {Tensor(), Tensor()};
+  const auto r = RotaryFn::apply(maybe(q), maybe(k), c, sign);
+  return {q.defined() ? r.front() : Tensor(), k.defined() ? r.back() : Tensor()};
+}
+
+std::tuple<Tensor, OptTensor> rotary_embedding(const Tensor& q, const OptTensor& k_opt, const OptTensor& positions, int64_t first,
+                                               const Tensor& inv_freq, bool interleaved, double scale) {
+  const char* name = "rotary_embedding";
+  const Tensor k = opt(k_opt);
+  HOST_ASSERT(q.dim() == 4 && (!k.defined() || k.dim() == 4), name, ": q and k must have four dimensions");
+  need_bf16(name, q);
+  if (k.defined()) need_bf16(name, k);
+  const int64_t B = q.size(0), T = q.size(1), D = q.size(3);
+  HOST_ASSERT(D % 16 == 0 && D >= 16 && D <= 1024, name, ": the head dim (", D, ") must be a multiple of 16 up to 1024");
+  HOST_ASSERT(!k.defined() || (k.size(0) == B && k.size(1) == T && k.size(3) == D), name, ": k ", k.defined() ? k.sizes() : q.sizes(),
+              " does not go with q ", q.sizes());
+  HOST_ASSERT(first >= -2147483647 && first <= 2147483647, name, ": first position out of range");
+  const Turn c{opt(positions), inv_freq, first, interleaved, scale};
+  check_turn(name, c, q, B, T, D, false);
+  same_device(name, q, {&k});
+  auto [qo, ko] = rotary_apply(q, k, c, 1.0);
+  return {qo, maybe(ko)};
+}
+
+// ---- the pages, their table and the sequences' lengths ------------------------------------------
+struct Pages {
+  int64_t pages, H, D, B, max_pages, seq_len;
+  Tensor lengths;
+};
+
+Pages check_pages(const char* name, const Tensor& like, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table,
+                  const py::object& length, const char* what, int64_t least) {
+  need_bf16(name, k_pages);
+  need_bf16(name, v_pages);
+  HOST_ASSERT(k_pages.dim() == 4 && k_pages.size(2) == 64 && v_pages.sizes() == k_pages.sizes() && k_pages.is_contiguous() &&
+                  v_pages.is_contiguous(),
+              name, ": k_pages ", k_pages.sizes(), " and v_pages ", v_pages.sizes(), " must be contiguous (pages, H, 64, D)");
+  Pages p{k_pages.size(0), k_pages.size(1), k_pages.size(3), like.size(0), 0, 0, Tensor()};
+  HOST_ASSERT(table.dim() == 2 && table.scalar_type() == at::kInt && table.size(0) == p.B && table.is_contiguous(), name,
+              ": page_table must be a contiguous int32 (", p.B, ", max_pages) tensor");
+  p.max_pages = table.size(1);
+  HOST_ASSERT(p.pages > 0 && p.H > 0 && p.max_pages > 0 && p.max_pages <= (1 << 24), name, ": no pages");
+  if (THPVariable_Check(length.ptr())) {
+    p.lengths = length.cast<Tensor>();
+    HOST_ASSERT(p.lengths.scalar_type() == at::kInt && p.lengths.sizes() == at::IntArrayRef({p.B}), name, ": ", what,
+                " must be an int or an int32 tensor of ", p.B, " lengths");
+    if (!p.lengths.is_cuda()) throw std::runtime_error(c10::str(name, ": tensors must live on the GPU (got ", p.lengths.device().str(), ")"));
+    p.lengths = p.lengths.contiguous();
+  } else {
+    p.seq_len = length.cast<int64_t>();
+    HOST_ASSERT(p.seq_len >= least && p.seq_len <= p.max_pages * 64, name, ": ", what, " ", p.seq_len, " must be between ", least,
+                " and the page table's ", p.max_pages * 64);
+  }
+  same_device(name, like, {&k_pages, &v_pages, &table, &p.lengths});
+  return p;
+}
+
+Tensor paged_append(const Tensor& k, const Tensor& v, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table,
+                    const py::object& seq_len, const OptTensor& q_opt, const OptTensor& inv_freq, const OptTensor& positions,
+                    bool interleaved, double scale) {
+  const char* name = "paged_append";
+  const Tensor q = opt(q_opt);
+  HOST_ASSERT(k.dim() == 4 && v.sizes() == k.sizes(), name, ": k ", k.sizes(), " and v ", v.sizes(), " must be (B, T, H, D)");
+  need_bf16(name, k);
+  need_bf16(name, v);
+  const int64_t B = k.size(0), T = k.size(1), H = k.size(2), D = k.size(3);
+  const Pages p = check_pages(name, k, k_pages, v_pages, table, seq_len, "seq_len", T);
+  HOST_ASSERT(p.H == H && p.D == D, name, ": pages of ", p.H, " heads of ", p.D, " for keys ", k.sizes());
+  HOST_ASSERT(D % 16 == 0 && D >= 16 && D <= 1024, name, ": the head dim (", D, ") must be a multiple of 16 up to 1024");
+  const Turn c{opt(positions), opt(inv_freq), 0, interleaved, scale};
+  if (c.inv_freq.defined()) check_turn(name, c, k, B, T, D, true);
+  HOST_ASSERT(c.inv_freq.defined() || !(c.positions.defined() || q.defined()), name,
+              ": q and positions are for the rotation: inv_freq is missing");
+  Tensor qo;
+  int64_t HQ = 0;
+  if (q.defined()) {
+    HOST_ASSERT(q.dim() == 4 && q.size(0) == B && q.size(1) == T && q.size(3) == D, name, ": q ", q.sizes(),
+                " does not go with k ", k.sizes());
+    need_bf16(name, q);
+    HQ = q.size(2);
+    qo = new_tensor(q.sizes(), q, q.scalar_type());
+  }
+  same_device(name, k, {&q, &v});
+  if (B * T * H == 0) return qo;
+  const c10::DeviceGuard on(k.device());
+  const Tensor ks = strided_rows(k), vs = strided_rows(v), qs = HQ ? strided_rows(q) : Tensor();
+  const Tensor pos = c.positions.defined() ? c.positions.contiguous() : Tensor();
+  HILS_CALL(hils_paged_append, cptr(qs), cptr(ks), cptr(vs), HQ ? mptr(qo) : nullptr, mptr(k_pages), mptr(v_pages), iptr(table),
+            iptr(p.lengths), cptr(pos), cptr(c.inv_freq), (size_t)(HQ ? qs.stride(0) : 0), (size_t)(HQ ? qs.stride(1) : 0),
+            (size_t)(HQ ? qs.stride(2) : 0), ROW_STRIDES(ks), ROW_STRIDES(vs), i32(B), i32(T), i32(HQ), i32(H), i32(D),
+            i32(c.inv_freq.defined() ? 2 * c.inv_freq.numel() : 0), (int)interleaved,
+            (int)(pos.defined() && pos.scalar_type() == at::kLong),
+            (int)(c.inv_freq.defined() && c.inv_freq.scalar_type() == at::kDouble), i32(p.max_pages), i32(p.pages),
+            i32(p.seq_len), (float)scale);
+  return qo;
+}
+
+std::tuple<Tensor, Tensor> paged_flex_attn(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table,
+                                           const py::object& seq_len, int64_t window, const OptTensor& parents_opt,
+                                           bool mask_lmk, bool expand, std::optional<double> sm_scale) {
+  const char* name = "paged_flex_attn";
+  HOST_ASSERT(q.dim() == 4, name, ": q must have four dimensions");
+  need_bf16(name, q);
+  const int64_t B = q.size(0), T = q.size(1), HQ = q.size(2), D = q.size(3);
+  const Pages p = check_pages(name, q, k_pages, v_pages, table, seq_len, "seq_len", T);
+  HOST_ASSERT(p.D == D && (D == 64 || D == 128), name, ": q heads of ", D, ", pages of ", p.D, ": both must be 64 or 128");
+  HOST_ASSERT(HQ % p.H == 0 && HQ > 0, name, ": H_q (", HQ, ") must be a multiple of H_kv (", p.H, ")");
+  HOST_ASSERT(window >= 1 && window <= 2147483647, name, ": window_size must be positive");
+  const double scale = scale_of(sm_scale, D);
+  HOST_ASSERT(scale > 0 && std::isfinite(scale), name, ": sm_scale must be positive and finite");
+  Tensor parents = opt(parents_opt);
+  if (parents.defined()) {
+    HOST_ASSERT(parents.scalar_type() == at::kInt && (parents.sizes() == at::IntArrayRef({T}) || parents.sizes() == at::IntArrayRef({B, T})),
+                name, ": parents must be an int32 tensor (T) or (B, T)");
+    HOST_ASSERT(T <= 256, name, ": a tree has at most 256 tokens (got ", T, ")");
+    if (!parents.is_cuda()) throw std::runtime_error(c10::str(name, ": tensors must live on the GPU (got ", parents.device().str(), ")"));
+    same_device(name, q, {&parents});
+    parents = parents.contiguous();
+  }
+  Tensor o = new_tensor({B, T, HQ, D}, q, q.scalar_type());
+  Tensor lse = new_tensor({B, T, HQ}, q, at::kFloat);
+  if (B * T == 0) return {o, lse};
+  const c10::DeviceGuard on(q.device());
+  const Tensor qs = strided_rows(q);
+  const int b = i32(B), t = i32(T), hq = i32(HQ), h = i32(p.H), d = i32(D), w = i32(window), mp = i32(p.max_pages);
+  const Tensor ws = workspace(hils_paged_attn_workspace(b, t, hq, h, d, w, mp), q);
+  HILS_CALL(hils_paged_attn, cptr(qs), cptr(k_pages), cptr(v_pages), iptr(table), iptr(p.lengths), iptr(parents), mptr(o),
+            mfptr(lse), mptr(ws), bytes(ws), ROW_STRIDES(qs), b, t, hq, h, d, mp, i32(p.pages), i32(p.seq_len),
+            (int)(parents.defined() && parents.dim() == 2), w, (int)mask_lmk, (int)expand, (float)scale);
+  return {o, lse};
+}
+
+void paged_accept(const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const py::object& base_len,
+                  const Tensor& path) {
+  const char* name = "paged_accept";
+  HOST_ASSERT(path.dim() == 2 && path.scalar_type() == at::kInt, name, ": path must be an int32 (B, n) tensor");
+  const Pages p = check_pages(name, path, k_pages, v_pages, table, base_len, "base_len", 0);
+  const int64_t n = path.size(1);
+  HOST_ASSERT(n <= 256, name, ": a path has at most 256 tokens (got ", n, ")");
+  HOST_ASSERT(p.D % 8 == 0, name, ": the head dim (", p.D, ") must be a multiple of 8");
+  if (n == 0 || p.B == 0) return;
+  const c10::DeviceGuard on(path.device());
+  const Tensor way = path.contiguous();
+  HILS_CALL(hils_paged_accept, mptr(k_pages), mptr(v_pages), iptr(table), iptr(p.lengths), iptr(way), i32(p.B), i32(n), i32(p.H),
+            i32(p.D), i32(p.max_pages), i32(p.pages), i32(p.seq_len));
+}
+
+void copy_pages(const std::vector<Tensor>& pools, const Tensor& src, const Tensor& dst) {
+  const char* name = "copy_pages";
+  HOST_ASSERT(!pools.empty() && pools.size() <= 8, name, ": 1 to 8 pools (got ", pools.size(), ")");
+  const at::ScalarType dt = src.scalar_type();
+  if ((dt != at::kInt && dt != at::kLong) || dst.scalar_type() != dt)
+    throw py::type_error(c10::str(name, ": src and dst must both be int32 or int64"));
+  HOST_ASSERT(src.dim() == 1 && src.sizes() == dst.sizes(), name, ": src ", src.sizes(), " and dst ", dst.sizes(),
+              " must be vectors of one length");
+  void* at_[8];
+  size_t size[8];
+  for (size_t i = 0; i < pools.size(); ++i) {
+    const Tensor& t = pools[i];
+    if (!t.is_cuda()) throw std::runtime_error(c10::str(name, ": tensors must live on the GPU (got ", t.device().str(), "); this package has no CPU path"));
+    HOST_ASSERT(t.dim() >= 1 && t.is_contiguous() && t.size(0) == pools[0].size(0), name, ": pools must be contiguous and have ",
+                pools[0].size(0), " pages each (got ", t.sizes(), ")");
+    HOST_ASSERT(t.numel() > 0, name, ": a pool is empty");
+    at_[i] = t.data_ptr();
+    size[i] = t.nbytes() / (size_t)t.size(0);
+    same_device(name, pools[0], {&t});
+  }
+  same_device(name, pools[0], {&src, &dst});
+  if (src.numel() == 0) return;
+  const c10::DeviceGuard on(pools[0].device());
+  const Tensor from = src.contiguous(), to = dst.contiguous();
+  HILS_CALL(hils_copy_pages, at_, size, cptr(from), cptr(to), (int)pools.size(), i32(from.numel()), i32(pools[0].size(0)),
+            (int)(dt == at::kLong));
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_hils_host, m) {
@@ -879,4 +1148,9 @@ PYBIND11_MODULE(_hils_host, m) {
   m.def("decode_step", &decode_step);
   m.def("paged_step", &paged_step);
   m.def("chunk_log_z", &chunk_log_z);
+  m.def("rotary_embedding", &rotary_embedding);
+  m.def("paged_append", &paged_append);
+  m.def("paged_flex_attn", &paged_flex_attn);
+  m.def("paged_accept", &paged_accept);
+  m.def("copy_pages", &copy_pages);
 }

@@ -61,6 +61,12 @@ SIGNATURES = {
     "hils_swa_bwd_workspace": [_I] * 7,
     "hils_swa_bwd_ws": [_P] * 11 + [_I] * 10 + [_F, _P, _Z, _P],
     "hils_swa_bwd": [_P] * 11 + [_I] * 10 + [_F, _P],
+    "hils_rotary": [_P] * 6 + [_Z] * 6 + [_I] * 11 + [_F, _F, _P],
+    "hils_paged_append": [_P] * 10 + [_Z] * 9 + [_I] * 12 + [_F, _P],
+    "hils_paged_attn_workspace": [_I] * 7,
+    "hils_paged_attn": [_P] * 9 + [_Z] * 4 + [_I] * 12 + [_F, _P],
+    "hils_paged_accept": [_P] * 5 + [_I] * 7 + [_P],
+    "hils_copy_pages": [_P] * 4 + [_I] * 4 + [_P],
 }
 
 _lib = None

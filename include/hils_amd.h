@@ -452,6 +452,65 @@ int hils_norm_rope_pool_bwd_ws(const void* x, const void* norm_weight, const voi
                                void* workspace, size_t workspace_bytes, int B, int L, int H, int D, int S,
                                int table_per_batch, float eps, void* stream);
 
+/* ---- rotary positions by position -------------------------------------------------------- */
+
+/* y = R(position) x for q (B,T,HQ,D) and, with H > 0, k (B,T,H,D), bf16, any strides (elements, multiples of 8; the features
+ * contiguous), into q_out, k_out (contiguous).  The first rotary_dim features are pairs, features i and i + rotary_dim / 2 or
+ * (interleaved) 2i and 2i + 1: y1 = scale (x1 cos a - x2 sin a), y2 = scale (x2 cos a + x1 sin a), a = position *
+ * inv_freq[i]; the others pass through.  inv_freq (rotary_dim / 2) fp32 or (inv_freq_64) fp64; positions int32 or
+ * (positions_64) int64, (T) or (positions_per_batch) (B,T), NULL: first_position + t.  Angles are formed in fp64 turns, the
+ * rotation in fp32, rounded once.  sin_sign = -1 is the backward (q, k then hold the gradients of q_out, k_out).
+ * D and rotary_dim multiples of 16, D <= 1024. */
+int hils_rotary(const void* q, const void* k, void* q_out, void* k_out, const void* positions, const void* inv_freq,
+                size_t q_batch_stride, size_t q_token_stride, size_t q_head_stride, size_t k_batch_stride,
+                size_t k_token_stride, size_t k_head_stride, int B, int T, int HQ, int H, int D, int rotary_dim,
+                int interleaved, int positions_64, int positions_per_batch, int first_position, int inv_freq_64,
+                float scale, float sin_sign, void* stream);
+
+/* ---- new and drafted tokens on a paged cache ---------------------------------------------- */
+
+/* Layouts of the paged cache as above: k_pages, v_pages (num_pages,H,64,D) bf16, page_table (B,max_pages) int32, chunk c of a
+ * sequence -> page (negative or >= num_pages: not mapped; nothing is written there and nobody sees what would lie there).
+ * lengths (B) int32: tokens of every sequence, the T new ones included; NULL: seq_len for all.  A sequence shorter than T
+ * takes no part.
+ *
+ * hils_paged_append: keys and values (B,T,H,D) of the last T tokens (slots length - T ..) into their pages, and q (B,T,HQ,D)
+ * into q_out (HQ = 0: none).  With rotary_dim > 0 q and k are rotated as by hils_rotary, at positions (B,T), NULL: the
+ * token's slot.  Nothing else of the pages is written.  D a multiple of 16, <= 1024. */
+int hils_paged_append(const void* q, const void* k, const void* v, void* q_out, void* k_pages, void* v_pages,
+                      const int32_t* page_table, const int32_t* lengths, const void* positions, const void* inv_freq,
+                      size_t q_batch_stride, size_t q_token_stride, size_t q_head_stride, size_t k_batch_stride,
+                      size_t k_token_stride, size_t k_head_stride, size_t v_batch_stride, size_t v_token_stride,
+                      size_t v_head_stride, int B, int T, int HQ, int H, int D, int rotary_dim, int interleaved,
+                      int positions_64, int inv_freq_64, int max_pages, int num_pages, int seq_len, float scale,
+                      void* stream);
+/* Local branch for the last T tokens of every sequence, straight on the pages: hils_swa_fwd on a cache (chunk 64), and for T
+ * drafted tokens that form a tree.  parents (T) or (parents_per_batch) (B,T) int32: the token that a drafted one follows,
+ * an earlier one, -1: the last committed token; NULL: a chain.  With base = length - T token t sits at position
+ * p = base + depth(t) and sees the committed tokens from left(p) on (left(p) = p - window + 1, moved to its chunk's first
+ * token with expand_to_chunk) and of the new ones itself and its ancestors at positions from left(p) on; with mask_lmk none
+ * at a chunk's last position.  A token with a parent that is no earlier token, and those that follow it, see nothing (the
+ * padding of a ragged batch of trees).  q (B,T,HQ,D) with any strides (multiples of 8 elements); o (B,T,HQ,D) bf16, lse
+ * (B,T,HQ) fp32 in natural-log units; rows that see nothing: o = 0, lse = -inf.  What a row does not see does not reach
+ * it, whatever lies there.  D in {64,128}, any HQ/H, T <= 256 with parents, sm_scale > 0.
+ * workspace: hils_paged_attn_workspace bytes (0: none): shares of the keys that several workgroups have are added up there. */
+size_t hils_paged_attn_workspace(int B, int T, int HQ, int H, int D, int window, int max_pages);
+int hils_paged_attn(const void* q, const void* k_pages, const void* v_pages, const int32_t* page_table,
+                    const int32_t* lengths, const int32_t* parents, void* o, float* lse, void* workspace,
+                    size_t workspace_bytes, size_t q_batch_stride, size_t q_token_stride, size_t q_head_stride, int B,
+                    int T, int HQ, int H, int D, int max_pages, int num_pages, int seq_len, int parents_per_batch,
+                    int window, int mask_lmk, int expand_to_chunk, float sm_scale, void* stream);
+/* Accepted drafts to the front: the keys and values at slots base + path[b][i] move to base + i, for the longest strictly
+ * growing start of path[b] (a negative entry ends it).  path (B,n) int32, n <= 256; bases (B) int32, NULL: base for all.
+ * The pages of the slots from base on must belong to the one sequence. */
+int hils_paged_accept(void* k_pages, void* v_pages, const int32_t* page_table, const int32_t* bases, const int32_t* path,
+                      int B, int n, int H, int D, int max_pages, int num_pages, int base, void* stream);
+/* pools[p][dst[i]] = pools[p][src[i]] for every i, pools of num_pages pages of page_bytes[p] bytes each, up to eight (pools
+ * and page_bytes are host arrays of n_pools).  src, dst (n) int32 or (indices_64) int64 on the device; a pair with an index
+ * out of range is left out.  A dst must be no other pair's src or dst. */
+int hils_copy_pages(void** pools, const size_t* page_bytes, const void* src, const void* dst, int n_pools, int n,
+                    int num_pages, int indices_64, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
