@@ -231,8 +231,8 @@ paged_attn_rows(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, cons
   constexpr int AREA = 32 * VP > ROWS * OP * 4 ? 32 * VP : ROWS * OP * 4;
   __shared__ __align__(16) unsigned char area_s[NWV * AREA];
   __shared__ float m_s[NWV][ROWS], l_s[NWV][ROWS];
-  __shared__ int par_s[TREE ? PA_MAX_TREE : 1], left_s[ROWS], odd_s;
-  __shared__ unsigned mask_s[TREE ? ROWS * PA_WORDS : 1];
+  __shared__ int par_s[TREE ? PA_MAX_TREE : 1], left_s[ROWS];
+  __shared__ unsigned mask_s[TREE ? ROWS * PA_WORDS : 1], odd_s;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, j = lane >> 4;
@@ -375,7 +375,7 @@ paged_attn_rows(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, cons
   {
     // two units' loads in flight; past the last unit the same one is asked for again and not worked on
     pa_u4 ka[2][KS], va[VI], kc[2][KS], vc[VI];
-    int n_mine = u1 > u0 + wave ? (u1 - u0 - wave + NWV - 1) / NWV : 0, done = 0;
+    int n_mine = u1 > u0 + wave ? (u1 - u0 - wave + NWV - 1) / NWV : 0;
     auto page_at = [&](int i) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(pages_of, i & 63); };
     int pg_a = page_at(0), pg_c;
     if (n_mine > 0) issue(ka, va, pg_a, (u0 + wave) & 1);
@@ -394,21 +394,26 @@ paged_attn_rows(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, cons
       vspan[rt] = some ? (unsigned)(last - lo) : 0u;
       if (TREE) mrow[rt] = mask_s + (live ? i : 0) * PA_WORDS;
     }
-    while (done < n_mine) {
-      const int u = u0 + wave + done * NWV;
-      const bool more = done + 1 < n_mine;
-      if (((done + 1) & 63) == 0 && more) ask_pages(u + NWV);
-      pg_c = more ? page_at(done + 1) : pg_a;
-      issue(kc, vc, pg_c, (more ? u + NWV : u) & 1);
+    // (the queries are here from now on: waited for inside the loop, the unit under way would be waited for with them)
+#pragma unroll
+    for (int rt = 0; rt < NR; ++rt)
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qb[rt][ks]));
+    auto next_page = [&](int i) __attribute__((always_inline)) {  // page of this wavefront's unit i, asked for 64 at a time
+      if ((i & 63) == 0) ask_pages(u0 + wave + i * NWV);
+      return page_at(i);
+    };
+    int u = u0 + wave, i = 0;
+    for (; i + 1 < n_mine; i += 2, u += 2 * NWV) {
+      pg_c = next_page(i + 1);
+      issue(kc, vc, pg_c, (u + NWV) & 1);
       if ((unsigned)pg_a < (unsigned)dm.num_pages) unit(ka, va, u);
-      if (++done >= n_mine) break;
-      const bool more2 = done + 1 < n_mine;
-      if (((done + 1) & 63) == 0 && more2) ask_pages(u + 2 * NWV);
-      pg_a = more2 ? page_at(done + 1) : pg_c;
-      issue(ka, va, pg_a, (more2 ? u + 2 * NWV : u + NWV) & 1);
+      const bool more = i + 2 < n_mine;  // (else the last one is asked for again and not worked on)
+      pg_a = more ? next_page(i + 2) : pg_c;
+      issue(ka, va, pg_a, (more ? u : u + NWV) & 1);
       if ((unsigned)pg_c < (unsigned)dm.num_pages) unit(kc, vc, u + NWV);
-      ++done;
     }
+    if (i < n_mine && (unsigned)pg_a < (unsigned)dm.num_pages) unit(ka, va, u);
   }
   // park the partial results: accumulator register i of tile mt in lane (row = col, j) is feature mt*16 + 4j + i
   __builtin_amdgcn_wave_barrier();
@@ -445,12 +450,12 @@ paged_attn_rows(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, cons
     const long row = ((long)b * dm.T + t) * dm.HQ + hk * dm.G + g;
     paged_store4<D>(dm, out, row, share, d4, x, M, L);
     const float all = (x[0] + x[1]) + (x[2] + x[3]);  // (no finite number if one of them is none)
-    if (!(fabsf(all) < INFINITY)) atomicOr(&odd_s, NR == 1 ? 1 << rr : -1);
+    if (!(fabsf(all) < INFINITY)) atomicOr(&odd_s, 1u << rr);
   }
   __syncthreads();
   if (const unsigned odd = odd_s; odd != 0) {
     for (int rr = wave; rr < r1 - r0; rr += NWV) {
-      if (NR == 1 && !(odd >> rr & 1)) continue;
+      if (!(odd >> rr & 1)) continue;
       const int r = r0 + rr, t = hils_udiv(r, dm.G, dm.g_magic), g = r - t * dm.G;
       const long row = ((long)b * dm.T + t) * dm.HQ + hk * dm.G + g;
       int left = TREE ? left_s[t - t0] : paged_left(sp.base + t, dm);
@@ -586,6 +591,12 @@ paged_attn_tiles(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, con
     const int row = 4 * j + (col >> 2);
     v_off[dt] = (unsigned)(row * RP + ((dt * 2 + (col >> 1 & 1)) ^ (row & (SEG - 1))) * 16 + (col & 1) * 8);
   }
+
+  // (the queries are here from now on: waited for inside the loop, the page under way would be waited for with them)
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qa[rt][ks]));
 
   auto tile_step = [&](int p, const unsigned char* k_s) __attribute__((always_inline)) {
     const unsigned char* v_s = k_s + TILE;
@@ -779,13 +790,13 @@ struct PagedPlan {
 static PagedPlan paged_plan(int B, int T, int HQ, int H, int window, int max_pages) {
   PagedPlan pl;
   const int rows = T * (HQ / H);
-  pl.tiles = rows > 64;
-  pl.nr = rows > 16 ? 2 : 1;
-  const int per = pl.tiles ? 128 : 16 * pl.nr;
-  pl.n_blk = (rows + per - 1) / per;
   // pages of the longest range a workgroup can have
   const long seen = (long)window + (T < 128 ? T : 128) + 2 * PA_PAGE - 3;
   const int pages = (int)(seen / PA_PAGE < max_pages ? seen / PA_PAGE : max_pages);
+  pl.tiles = rows > 64 && (long)((rows + 31) / 32) * H * B * pages > 2048;
+  pl.nr = rows > 16 ? 2 : 1;
+  const int per = pl.tiles ? 128 : 16 * pl.nr;
+  pl.n_blk = (rows + per - 1) / per;
   const long wgs = (long)pl.n_blk * H * B;
   const long want = (2l * hils_device_cus() + wgs - 1) / wgs;  // two workgroups a compute unit
   const int least = 8;                                         // pages of a share

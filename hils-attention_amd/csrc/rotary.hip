@@ -6,7 +6,9 @@
 // the other D - R features pass through.  The backward is the same with -a (`sign`).
 //
 // The angle of a far position has lost its fraction of a turn in fp32 (position 10^6, inv_freq 1: steps of 0.06), so it is
-// formed in turns in fp64, reduced to [-1/2, 1/2] there, and only then rounded; the rotation is fp32, rounded once to bf16.
+// formed in turns in fp64 and reduced to [-1/2, 1/2] there; the rotation is fp64 too (fp32's rate on this chip, and the kernel
+// waits for memory), so that what is rounded to bf16, once, is the exact value: a key in the cache is the same whatever
+// computed it.
 // Bound by HBM: q and k in and out.  A workgroup owns a few tokens of all heads; their R/2 angles each are worked out
 // once, into LDS, for all heads (an angle costs some 60 instructions: per head they would be most of the kernel).  A
 // thread's unit is 16 features that go together: two 16-byte pieces in and out, four units' loads in flight.
@@ -25,68 +27,89 @@ struct RotaryDims {
   const int32_t* lengths;                     // (B) or null: seq_len
 };
 
-#define ROT_UN 4
+#ifndef ROT_UN
+#define ROT_UN 2
+#define ROT_WAVES 4
+#endif
 
-__global__ void __launch_bounds__(256)
+// Eight pairs of a unit.  The rounding fp64 -> fp32 -> bf16 differs from the one to bf16 only where the first lands halfway
+// between two bf16 values: true if some value did (about one in 65536), and with FIX such a value goes the way it came from.
+template <bool INTERLEAVED, bool FIX>
+__device__ __forceinline__ bool rotary_turn(const uint4 lo, const uint4 hi, const double* c, const double* s, uint4& out_lo,
+                                            uint4& out_hi) {
+  float a[8], b[8], y1[8], y2[8];
+  unpack8(lo, a);
+  unpack8(hi, b);
+  bool tie = false;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const double x1 = INTERLEAVED ? (i < 4 ? a[2 * i & 7] : b[2 * i & 7]) : a[i];
+    const double x2 = INTERLEAVED ? (i < 4 ? a[(2 * i + 1) & 7] : b[(2 * i + 1) & 7]) : b[i];
+    const double d1 = fma(x1, c[i], -(x2 * s[i])), d2 = fma(x2, c[i], x1 * s[i]);
+    float f1 = (float)d1, f2 = (float)d2;
+    if (FIX) {
+      auto fix = [](double d, float f) {
+        unsigned u = __float_as_uint(f);
+        const double back = f;
+        if ((u & 0xffffu) == 0x8000u && d != back) u += (d > back) == (f > 0.f) ? 1u : -1u;
+        return __uint_as_float(u);
+      };
+      f1 = fix(d1, f1);
+      f2 = fix(d2, f2);
+    } else {
+      tie |= (__float_as_uint(f1) & 0xffffu) == 0x8000u;
+      tie |= (__float_as_uint(f2) & 0xffffu) == 0x8000u;
+    }
+    y1[i] = f1;
+    y2[i] = f2;
+  }
+  unsigned* wl = (unsigned*)&out_lo;
+  unsigned* wh = (unsigned*)&out_hi;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    wl[i] = INTERLEAVED ? pack_bf2(y1[i], y2[i]) : pack_bf2(y1[2 * i], y1[2 * i + 1]);
+    wh[i] = INTERLEAVED ? pack_bf2(y1[4 + i], y2[4 + i]) : pack_bf2(y2[2 * i], y2[2 * i + 1]);
+  }
+  return tie;
+}
+
+template <bool INTERLEAVED, bool APPEND>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(ROT_WAVES)))
 rotary_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, const bf16_t* __restrict__ v,
               bf16_t* __restrict__ q_out, bf16_t* __restrict__ k_out, bf16_t* __restrict__ v_out, RotaryDims dm) {
-  extern __shared__ __align__(16) float rot_s[];
-  __shared__ int page_s[8], at_s[8], b_s[8], t_s[8];
-  const int half = dm.R / 2;
-  float* cos_s = rot_s;
-  float* sin_s = rot_s + dm.tpb * half;
+  extern __shared__ __align__(16) double rot_s[];
+  __shared__ long slot_s[8];  // place of a token's key in the pages, in rows of a pool's first head; -1: none
+  const int half = dm.R / 2, tid = threadIdx.x;
+  double* cos_s = rot_s;
+  double* sin_s = rot_s + dm.tpb * half;
   const long tok0 = (long)blockIdx.x * dm.tpb;
   const int n = dm.n_tok - tok0 < dm.tpb ? (int)(dm.n_tok - tok0) : dm.tpb;
-  const int tid = threadIdx.x;
-  if (tid < n) {
-    const long tok = tok0 + tid;
-    const int b = dm.m_tok ? (int)(tok / dm.T) : (int)tok, t = (int)(tok - (long)b * dm.T);
-    b_s[tid] = b;
-    t_s[tid] = t;
-    if (dm.append) {
-      const int slot = (dm.lengths ? dm.lengths[b] : dm.seq_len) - dm.T + t;
-      const int c = slot >> 6;
-      const int page = slot >= 0 && c < dm.max_pages ? dm.table[(long)b * dm.max_pages + c] : -1;
-      page_s[tid] = (unsigned)page < (unsigned)dm.num_pages ? page : -1;
-      at_s[tid] = slot;
-    }
-  }
-  __syncthreads();
-  for (int i = tid; i < n * half; i += 256) {
-    const int tk = i / half, f = i - tk * half;
-    double p;
-    if (dm.positions) {
-      const long at = (dm.pos_batch ? (long)b_s[tk] * dm.T : 0) + t_s[tk];
-      p = dm.pos_wide ? (double)((const int64_t*)dm.positions)[at] : (double)((const int32_t*)dm.positions)[at];
-    } else {
-      p = dm.append ? (double)at_s[tk] : (double)((long)dm.pos0 + t_s[tk]);
-    }
-    const double w = dm.freq_wide ? ((const double*)dm.inv_freq)[f] : (double)((const float*)dm.inv_freq)[f];
-    const double turns = p * (w * 0.15915494309189533577);  // 1 / (2 pi)
-    float sn, cs;
-    sincospif(2.f * (float)(turns - rint(turns)), &sn, &cs);
-    cos_s[i] = cs * dm.scale;
-    sin_s[i] = sn * dm.scale * dm.sign;
-  }
-  __syncthreads();
-  const int U = dm.D / 16, UR = dm.R / 16, NH = dm.HQ + dm.H + (dm.append ? dm.H : 0);
+  const int b0 = (int)((unsigned long)tok0 / (unsigned)dm.T), t0 = (int)(tok0 - (long)b0 * dm.T);
+  auto token = [&](int tk, int& b, int& t) __attribute__((always_inline)) {  // (a workgroup has up to eight tokens)
+    t = t0 + tk;
+    const int w = dm.T >= 8 ? t >= dm.T : (int)hils_udiv(t, dm.T, dm.m_tok);
+    b = b0 + w;
+    t -= w * dm.T;
+  };
+  const int U = dm.D / 16, UR = dm.R / 16, NH = dm.HQ + dm.H + (APPEND ? dm.H : 0);
   const int total = n * NH * U;
-  for (int e0 = tid; e0 < total; e0 += 256 * ROT_UN) {
-    uint4 lo[ROT_UN], hi[ROT_UN];
-    bf16_t* to[ROT_UN];
-    int gap[ROT_UN], tab[ROT_UN];
+  uint4 lo[ROT_UN], hi[ROT_UN];
+  bf16_t* to[ROT_UN];
+  int gap[ROT_UN], tab[ROT_UN];  // elements between a unit's pieces; its first angle, -1: not rotated
+  int late[ROT_UN];              // token whose place in the pages `to` waits for, -1: none
+  auto load = [&](int e0) __attribute__((always_inline)) {
 #pragma unroll
     for (int x = 0; x < ROT_UN; ++x) {
       const int e = e0 + 256 * x;
       to[x] = nullptr;
       gap[x] = 8;
-      tab[x] = -1;
+      tab[x] = late[x] = -1;
       lo[x] = hi[x] = make_uint4(0, 0, 0, 0);
       if (e < total) {
         const int r = hils_udiv(e, U, dm.m_unit), u = e - r * U;
         const int tk = hils_udiv(r, NH, dm.m_head);
-        int h = r - tk * NH;
-        const long b = b_s[tk], t = t_s[tk];
+        int h = r - tk * NH, b, t;
+        token(tk, b, t);
         const bf16_t* from;
         bool turn = u < UR;
         if (h < dm.HQ) {
@@ -98,53 +121,67 @@ rotary_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, const 
           h = is_v ? h - dm.H : h;
           turn = turn && !is_v;
           from = is_v ? v + b * dm.v_sb + t * dm.v_st + h * dm.v_sh : k + b * dm.k_sb + t * dm.k_st + h * dm.k_sh;
-          if (dm.append) {
-            const int page = page_s[tk];
-            bf16_t* pool = is_v ? v_out : k_out;
-            to[x] = page < 0 ? nullptr : pool + (((long)page * dm.H + h) * 64 + (at_s[tk] & 63)) * dm.D;
+          if (APPEND) {
+            to[x] = (is_v ? v_out : k_out) + (long)h * 64 * dm.D;
+            late[x] = tk;
           } else {
             to[x] = k_out + ((tok0 + tk) * dm.H + h) * dm.D;
           }
         }
-        const int first = turn && !dm.interleaved ? u * 8 : u * 16;
+        const int first = turn && !INTERLEAVED ? u * 8 : u * 16;
         if (turn) {
           tab[x] = tk * half + u * 8;
-          gap[x] = dm.interleaved ? 8 : half;
+          gap[x] = INTERLEAVED ? 8 : half;
         }
-        from += first;
-        if (to[x]) {
-          to[x] += first;
-          lo[x] = *(const uint4*)from;
-          hi[x] = *(const uint4*)(from + gap[x]);
-        }
+        to[x] += first;
+        lo[x] = *(const uint4*)(from + first);
+        hi[x] = *(const uint4*)(from + first + gap[x]);
       }
     }
+  };
+  load(tid);  // (under way while the angles are worked out)
+  if (APPEND && tid < n) {
+    int b, t;
+    token(tid, b, t);
+    const int slot = (dm.lengths ? dm.lengths[b] : dm.seq_len) - dm.T + t, c = slot >> 6;
+    const int page = slot >= 0 && c < dm.max_pages ? dm.table[(long)b * dm.max_pages + c] : -1;
+    slot_s[tid] = (unsigned)page < (unsigned)dm.num_pages ? (long)page * dm.H * 64 + (slot & 63) : -1;
+  }
+  for (int i = tid; i < n * half; i += 256) {
+    const int tk = i / half, f = i - tk * half;
+    int b, t;
+    token(tk, b, t);
+    double p;
+    if (dm.positions) {
+      const long at = (dm.pos_batch ? (long)b * dm.T : 0) + t;
+      p = dm.pos_wide ? (double)((const int64_t*)dm.positions)[at] : (double)((const int32_t*)dm.positions)[at];
+    } else {
+      p = APPEND ? (double)((dm.lengths ? dm.lengths[b] : dm.seq_len) - dm.T + t) : (double)((long)dm.pos0 + t);
+    }
+    const double w = dm.freq_wide ? ((const double*)dm.inv_freq)[f] : (double)((const float*)dm.inv_freq)[f];
+    const double turns = p * (w * 0.15915494309189533577);  // 1 / (2 pi)
+    double sn, cs;
+    sincospi(2.0 * (turns - rint(turns)), &sn, &cs);
+    cos_s[i] = cs * dm.scale;
+    sin_s[i] = sn * dm.scale * dm.sign;
+  }
+  __syncthreads();
+  for (int e0 = tid; e0 < total; e0 += 256 * ROT_UN) {
+    if (e0 != tid) load(e0);
 #pragma unroll
     for (int x = 0; x < ROT_UN; ++x) {
       if (!to[x]) continue;
       if (tab[x] >= 0) {
-        float a[8], b[8], c[8], s[8];
-        unpack8(lo[x], a);
-        unpack8(hi[x], b);
-        *(f32x4_t*)&c[0] = *(const f32x4_t*)&cos_s[tab[x]];
-        *(f32x4_t*)&c[4] = *(const f32x4_t*)&cos_s[tab[x] + 4];
-        *(f32x4_t*)&s[0] = *(const f32x4_t*)&sin_s[tab[x]];
-        *(f32x4_t*)&s[4] = *(const f32x4_t*)&sin_s[tab[x] + 4];
-        unsigned* wl = (unsigned*)&lo[x];
-        unsigned* wh = (unsigned*)&hi[x];
-        if (dm.interleaved) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            wl[i] = pack_bf2(a[2 * i] * c[i] - a[2 * i + 1] * s[i], a[2 * i + 1] * c[i] + a[2 * i] * s[i]);
-            wh[i] = pack_bf2(b[2 * i] * c[4 + i] - b[2 * i + 1] * s[4 + i], b[2 * i + 1] * c[4 + i] + b[2 * i] * s[4 + i]);
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            wl[i] = pack_bf2(a[2 * i] * c[2 * i] - b[2 * i] * s[2 * i], a[2 * i + 1] * c[2 * i + 1] - b[2 * i + 1] * s[2 * i + 1]);
-            wh[i] = pack_bf2(b[2 * i] * c[2 * i] + a[2 * i] * s[2 * i], b[2 * i + 1] * c[2 * i + 1] + a[2 * i + 1] * s[2 * i + 1]);
-          }
-        }
+        const double* c = cos_s + tab[x];
+        const double* sn = sin_s + tab[x];
+        const uint4 l0 = lo[x], h0 = hi[x];
+        if (rotary_turn<INTERLEAVED, false>(l0, h0, c, sn, lo[x], hi[x]))
+          rotary_turn<INTERLEAVED, true>(l0, h0, c, sn, lo[x], hi[x]);
+      }
+      if (late[x] >= 0) {
+        const long at = slot_s[late[x]];
+        if (at < 0) continue;
+        to[x] += at * dm.D;
       }
       *(uint4*)to[x] = lo[x];
       *(uint4*)(to[x] + gap[x]) = hi[x];
@@ -159,14 +196,17 @@ static int rotary_launch(const char* who, RotaryDims& dm, const void* q, const v
   long tpb = dm.n_tok / (4l * hils_device_cus());
   const int most = 2048 / units;
   tpb = tpb < most ? tpb : most;
+  tpb = dm.R == 0 || tpb < 4096 / dm.R ? tpb : 4096 / dm.R;  // (tables of up to 32 KiB of LDS)
   dm.tpb = tpb < 1 ? 1 : tpb > 8 ? 8 : (int)tpb;
   dm.m_unit = hils_udiv_magic(dm.D / 16);
   dm.m_head = hils_udiv_magic(heads);
-  dm.m_tok = dm.T > 1;
+  dm.m_tok = hils_udiv_magic(dm.T);
   const long blocks = (dm.n_tok + dm.tpb - 1) / dm.tpb;
   HILS_REQUIRE(blocks <= 2147483647L && (long)dm.tpb * units * heads < (1l << 31), "%s: sizes too large for the grid", who);
-  hipLaunchKernelGGL(rotary_kernel, dim3((unsigned)blocks), dim3(256), (size_t)dm.tpb * dm.R * sizeof(float), st,
-                     (const bf16_t*)q, (const bf16_t*)k, (const bf16_t*)v, (bf16_t*)q_out, (bf16_t*)k_out, (bf16_t*)v_out, dm);
+  auto kern = dm.append ? (dm.interleaved ? rotary_kernel<true, true> : rotary_kernel<false, true>)
+                        : (dm.interleaved ? rotary_kernel<true, false> : rotary_kernel<false, false>);
+  hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), (size_t)dm.tpb * dm.R * sizeof(double), st, (const bf16_t*)q,
+                     (const bf16_t*)k, (const bf16_t*)v, (bf16_t*)q_out, (bf16_t*)k_out, (bf16_t*)v_out, dm);
   HILS_CHECK_LAUNCH(who);
   return HILS_OK;
 }

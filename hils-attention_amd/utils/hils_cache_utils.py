@@ -26,12 +26,14 @@ try:  # imported as part of the package ...
     from ..ops.chunk_attn_pool_tilelang import chunk_attn_pool, chunk_mean_pool
     from ..ops.hils_fwd_bwd_head import HiLS_block_M_head
     from ..ops.hils_glue import chunk_weights, decode_step, topk_chunk_weights
+    from ..ops.paged_cache import copy_pages, paged_accept, paged_append, paged_flex_attn
     from ..ops.topk_head_softmax import online_softmax_topk_head
 except ImportError:  # ... or with the package directory itself on sys.path (`from utils... import`)
     from ops import _cabi
     from ops.chunk_attn_pool_tilelang import chunk_attn_pool, chunk_mean_pool
     from ops.hils_fwd_bwd_head import HiLS_block_M_head
     from ops.hils_glue import chunk_weights, decode_step, topk_chunk_weights
+    from ops.paged_cache import copy_pages, paged_accept, paged_append, paged_flex_attn
     from ops.topk_head_softmax import online_softmax_topk_head
 
 
@@ -230,7 +232,12 @@ class HiLSPagedLayer:
     when ``update`` is given the chunks' prior queries ``mu_q``, the attention pool's entropy bias is
     kept too (and its pooled key replaces the mean unless ``chunk_pooling``).  All sequences of the batch
     have the same length (the kernels take one query offset, as the reference's do).  Pages come from a
-    free list, so the page order of a sequence is arbitrary."""
+    free list, so the page order of a sequence is arbitrary.
+
+    Sequences may share pages after ``fork``: a page counts its users, returns to the free list when the last one lets go
+    of it, and is copied before a sequence writes on a page that others use too.  ``draft`` appends tokens on trial, in a
+    chain or a tree; ``local_attend`` and ``hils_attend`` then are for them, and ``accept`` keeps a path of the tree and
+    drops the rest.  ``truncate`` and ``free`` give tokens up, ``compact`` gathers the pages in use at the front."""
 
     def __init__(self, num_pages, batch, max_pages_per_seq, num_kv_heads, head_dim, device,
                  num_q_heads=None, chunk_pooling=True, page_order=None, dtype=torch.bfloat16):
@@ -256,6 +263,11 @@ class HiLSPagedLayer:
         self.free_pages = order
         self.seq_len = 0
         self.pooled_chunks = 0
+        self._pages = [[] for _ in range(self.B)]  # the mapped part of the page table, on the host
+        self._users = [0] * self.num_pages         # sequences that a page belongs to
+        self.drafted = 0                           # tokens on trial behind the sequence
+        self._parents = None                       # (B or 1) lists of their parents, None: a chain
+        self._parents_dev = None
 
     @property
     def prior_b(self):
@@ -265,62 +277,250 @@ class HiLSPagedLayer:
     def get_seq_length(self):
         return self.seq_len
 
-    def update(self, key_states, value_states, mu_q=None):
+    # ---- pages -------------------------------------------------------------------------------------
+    def _take(self, have, need):
+        """Map chunks ``have`` .. ``need - 1`` of every sequence to free pages."""
+        if need <= have:
+            return
+        n_new = (need - have) * self.B
+        new = [self.free_pages.pop() for _ in range(n_new)]
+        for i, page in enumerate(new):  # chunk by chunk, the sequences in turn
+            self._pages[i % self.B].append(page)
+            self._users[page] = 1
+        self.page_table[:, have:need] = torch.tensor(new, dtype=torch.int32, device=self.page_table.device).view(
+            need - have, self.B).t()
+
+    def _give_back(self, pages):
+        for page in pages:
+            self._users[page] -= 1
+            if self._users[page] == 0:
+                self.free_pages.append(page)
+
+    def _keep_pages(self, tokens):
+        """Let go of the pages behind the first ``tokens`` tokens."""
+        keep = (tokens + self.S - 1) // self.S
+        had = max(len(p) for p in self._pages) if self._pages else 0
+        for b in range(self.B):
+            self._give_back(self._pages[b][keep:])
+            del self._pages[b][keep:]
+        if had > keep:
+            self.page_table[:, keep:had] = -1
+
+    def _pools(self):
+        return [p for p in (self.k_pages, self.v_pages, self.lmk_pages, self.prior_pages) if p is not None]
+
+    def _own_tail(self, tokens):
+        """Before a write behind ``tokens`` tokens: copies of the partly filled pages that other sequences use too."""
+        c = tokens // self.S
+        src, dst, who = [], [], []
+        for b in self._tail_sharers(tokens):
+            page = self._pages[b][c]
+            new = self.free_pages.pop()
+            self._users[page] -= 1
+            self._users[new] = 1
+            self._pages[b][c] = new
+            src.append(page), dst.append(new), who.append(b)
+        if src:
+            copy_pages(self._pools(), src, dst)
+            dev = self.page_table.device
+            self.page_table[torch.tensor(who, device=dev), c] = torch.tensor(dst, dtype=torch.int32, device=dev)
+
+    def _tail_sharers(self, tokens):
+        """The sequences that need a copy of their partly filled page: of its users all but the last."""
+        if tokens % self.S == 0:
+            return []
+        c, left, out = tokens // self.S, {}, []
+        for b in range(self.B):
+            page = self._pages[b][c]
+            left[page] = left.get(page, self._users[page]) - 1
+            if left[page]:
+                out.append(b)
+        return out
+
+    def _append(self, key_states, value_states, q, rotary):
+        """Keys and values behind the sequence, into pages of its own; the rotated q."""
+        B, T, H, D = key_states.shape
+        assert (B, H, D) == (self.B, self.H, self.D)
+        a, b_end, S = self.seq_len, self.seq_len + T, self.S
+        have, need = (a + S - 1) // S, (b_end + S - 1) // S
+        assert need <= self.max_pages, "the page table is too short for this sequence length"
+        copies = len(self._tail_sharers(a)) if T else 0
+        assert copies + (need - have) * B <= len(self.free_pages), "out of pages"
+        if copies:
+            self._own_tail(a)
+        self._take(have, need)
+        if self.k_pages.is_cuda and self.k_pages.dtype == torch.bfloat16 and D % 16 == 0 and D <= 1024:
+            return paged_append(key_states, value_states, self.k_pages, self.v_pages, self.page_table, b_end, q=q, **rotary)
+        # a cache in a type that the attention does not take is kept all the same
+        assert q is None and not rotary, "the rotation needs a bf16 cache on the GPU"
+        pos = torch.arange(a, b_end, device=self.k_pages.device)
+        pages = self.page_table[:, pos // S].long().unsqueeze(-1)        # (B, T, 1)
+        slots = (pos % S).view(1, T, 1).expand(B, T, 1)
+        hh = torch.arange(H, device=self.k_pages.device).view(1, 1, H)
+        self.k_pages[pages, hh, slots] = key_states
+        self.v_pages[pages, hh, slots] = value_states
+        return None
+
+    def _pool_full_chunks(self, mu_q):
+        """Chunk keys (and the prior bias) of the chunks that are full and have none yet."""
+        B, H, D, S = self.B, self.H, self.D, self.S
+        full = self.seq_len // S
+        if full <= self.pooled_chunks:
+            return
+        c0 = self.pooled_chunks
+        n = full - c0
+        pg = self.page_table[:, c0:full].long().reshape(-1)          # (B * n) pages, batch-major
+        kk = self.k_pages[pg]                                        # (B*n, H, 64, D), a copy
+        pooled = None
+        if self.chunk_pooling or mu_q is None:
+            # every (page, head) is a 64-token sequence of its own for the pooling kernel
+            pooled = chunk_mean_pool(kk.view(-1, S, 1, D), S).view(-1, H, D)
+        if mu_q is not None:
+            hq = mu_q.shape[2]
+            G = hq // H
+            assert mu_q.shape == (B, n, hq, D), f"mu_q shape {tuple(mu_q.shape)}"
+            assert self.prior_pages is not None, "construct the layer with num_q_heads to keep a prior bias"
+            assert c0 == 0 or self.has_prior, "the prior bias must be kept from the first chunk on"
+            lk, lb = _attention_pooled(mu_q.reshape(-1, 1, hq, D), kk.permute(0, 2, 1, 3).unsqueeze(1), H)
+            self.prior_pages[pg] = lb.reshape(-1, hq)
+            self.prior_hm[:, :, c0:full] = lb.view(B, n, H, G).permute(0, 2, 1, 3)
+            self.has_prior = True
+            if pooled is None:
+                assert hq == self.h_lmk, "attention-pooled chunk keys are per query head"
+                pooled = lk.reshape(-1, hq, D)
+        else:
+            assert not self.has_prior, "this cache keeps a prior bias: update() needs mu_q for new chunks"
+        assert pooled.shape[1] == self.h_lmk, (
+            "a layer built without chunk pooling keeps the attention pool's keys: update() needs mu_q")
+        pooled = pooled.to(self.lmk_pages.dtype)
+        self.lmk_pages[pg] = pooled
+        self.lmk_hm[:, :, c0:full] = pooled.view(B, n, self.h_lmk, D).permute(0, 2, 1, 3)
+        self.pooled_chunks = full
+
+    # ---- tokens ------------------------------------------------------------------------------------
+    def update(self, key_states, value_states, mu_q=None, q=None, **rotary):
         """Append (B, T, H, D) keys / values.  ``mu_q`` (B, new_full_chunks, h_q, D): the prior queries
         of the chunks this call completes; with it the entropy bias of the attention pool is kept and
         used by ``hils_attend`` (and the attention-pooled keys are the chunk keys unless
-        ``chunk_pooling``)."""
-        B, T, H, D = key_states.shape
-        assert (B, H, D) == (self.B, self.H, self.D)
-        S, dev = self.S, self.k_pages.device
-        a, b_end = self.seq_len, self.seq_len + T
-        need = (b_end + S - 1) // S
-        have = (a + S - 1) // S
-        assert need <= self.max_pages, "the page table is too short for this sequence length"
-        if need > have:
-            n_new = (need - have) * B
-            assert n_new <= len(self.free_pages), "out of pages"
-            new = torch.tensor([self.free_pages.pop() for _ in range(n_new)], dtype=torch.int32,
-                               device=dev).view(need - have, B).t()
-            self.page_table[:, have:need] = new
-        pos = torch.arange(a, b_end, device=dev)
-        pages = self.page_table[:, pos // S].long()                      # (B, T)
-        slots = (pos % S).view(1, T).expand(B, T)
-        hh = torch.arange(H, device=dev).view(1, 1, H)
-        self.k_pages[pages.unsqueeze(-1), hh, slots.unsqueeze(-1)] = key_states
-        self.v_pages[pages.unsqueeze(-1), hh, slots.unsqueeze(-1)] = value_states
-        self.seq_len = b_end
-        full = b_end // S
-        if full > self.pooled_chunks:
-            c0 = self.pooled_chunks
-            n = full - c0
-            pg = self.page_table[:, c0:full].long().reshape(-1)          # (B * n) pages, batch-major
-            kk = self.k_pages[pg]                                        # (B*n, H, 64, D), a copy
-            pooled = None
-            if self.chunk_pooling or mu_q is None:
-                # every (page, head) is a 64-token sequence of its own for the pooling kernel
-                pooled = chunk_mean_pool(kk.view(-1, S, 1, D), S).view(-1, H, D)
-            if mu_q is not None:
-                hq = mu_q.shape[2]
-                G = hq // H
-                assert mu_q.shape == (B, n, hq, D), f"mu_q shape {tuple(mu_q.shape)}"
-                assert self.prior_pages is not None, "construct the layer with num_q_heads to keep a prior bias"
-                assert c0 == 0 or self.has_prior, "the prior bias must be kept from the first chunk on"
-                lk, lb = _attention_pooled(mu_q.reshape(-1, 1, hq, D), kk.permute(0, 2, 1, 3).unsqueeze(1), H)
-                self.prior_pages[pg] = lb.reshape(-1, hq)
-                self.prior_hm[:, :, c0:full] = lb.view(B, n, H, G).permute(0, 2, 1, 3)
-                self.has_prior = True
-                if pooled is None:
-                    assert hq == self.h_lmk, "attention-pooled chunk keys are per query head"
-                    pooled = lk.reshape(-1, hq, D)
-            else:
-                assert not self.has_prior, "this cache keeps a prior bias: update() needs mu_q for new chunks"
-            assert pooled.shape[1] == self.h_lmk, (
-                "a layer built without chunk pooling keeps the attention pool's keys: update() needs mu_q")
-            pooled = pooled.to(self.lmk_pages.dtype)
-            self.lmk_pages[pg] = pooled
-            self.lmk_hm[:, :, c0:full] = pooled.view(B, n, self.h_lmk, D).permute(0, 2, 1, 3)
-            self.pooled_chunks = full
+        ``chunk_pooling``).  With ``inv_freq`` (and ``interleaved``, ``scale``, ``positions``, as for
+        ``paged_append``) the keys, and the queries ``q`` if given, are rotated on the way; returns the
+        rotated q."""
+        assert not self.drafted, "tokens are on trial: accept() first"
+        q = self._append(key_states, value_states, q, rotary)
+        self.seq_len += key_states.shape[1]
+        self._pool_full_chunks(mu_q)
+        return q
+
+    def draft(self, key_states, value_states, parents=None, q=None, **rotary):
+        """Append T tokens (B, T, H, D) on trial: nothing is pooled, the length stays.  ``parents``: for every token the
+        drafted one that it follows, an earlier one, or -1 for the last token of the sequence; T or (B, T) ints, on the host
+        (a tensor on the GPU is copied there, which waits for it); None: each follows the one before.  Rotation as in
+        ``update``, at the positions the tokens' depths give them."""
+        assert not self.drafted, "tokens are on trial: accept() first"
+        B, T = key_states.shape[:2]
+        assert T > 0, "draft() needs a token"
+        rows = None
+        if parents is not None:
+            parents = torch.as_tensor(parents).to("cpu", torch.int64)
+            assert tuple(parents.shape) in ((T,), (B, T)), f"parents {tuple(parents.shape)} for {T} tokens"
+            rows = parents.view(-1, T).tolist()
+            if any(not -1 <= p < t for row in rows for t, p in enumerate(row)):
+                raise ValueError("draft: a token's parent is an earlier drafted token or -1")
+        depths = self._depths(rows, T)
+        if rotary.get("inv_freq") is not None and rows is not None and rotary.get("positions") is None:
+            at = torch.tensor(depths, dtype=torch.int32) + self.seq_len
+            rotary = dict(rotary, positions=at.expand(B, T).contiguous().to(self.k_pages.device))
+        q = self._append(key_states, value_states, q, rotary)
+        self.drafted, self._parents, self._depth_rows = T, rows, depths
+        self._parents_dev = None if rows is None else torch.tensor(
+            rows if len(rows) > 1 else rows[0], dtype=torch.int32, device=self.k_pages.device)
+        return q
+
+    @staticmethod
+    def _depths(rows, T):
+        if rows is None:
+            return [list(range(T))]
+        out = []
+        for row in rows:
+            d = []
+            for p in row:
+                d.append(0 if p < 0 else d[p] + 1)
+            out.append(d)
+        return out
+
+    def accept(self, path=(), mu_q=None):
+        """Keep the drafted tokens ``path`` (n ints, or (B, n); a way down the tree from a token with parent -1) as the
+        sequence's next n tokens, drop the others.  As many for every sequence.  ``mu_q`` as in ``update``."""
+        assert self.drafted, "no tokens are on trial"
+        path = torch.as_tensor(path, dtype=torch.int64).to("cpu")
+        path = path.expand(self.B, -1) if path.dim() == 1 else path
+        assert path.dim() == 2 and path.shape[0] == self.B, f"path {tuple(path.shape)}"
+        n, T = path.shape[1], self.drafted
+        for b, way in enumerate(path.tolist()):
+            up = list(range(-1, T - 1)) if self._parents is None else self._parents[b % len(self._parents)]
+            if any(not 0 <= t < T for t in way) or any(up[t] != p for t, p in zip(way, [-1] + way)):
+                raise ValueError(f"accept: {way} is no way down the tree of sequence {b}")
+        if n and not torch.equal(path, torch.arange(n).expand(self.B, n)):
+            paged_accept(self.k_pages, self.v_pages, self.page_table, self.seq_len,
+                         path.to(self.k_pages.device, torch.int32))
+        self.drafted, self._parents, self._parents_dev, self._depth_rows = 0, None, None, None
+        self.seq_len += n
+        self._keep_pages(self.seq_len)
+        self._pool_full_chunks(mu_q)
+
+    def truncate(self, length):
+        """Give up the tokens behind the first ``length`` (and drafted ones)."""
+        assert 0 <= length <= self.seq_len, f"{length} of {self.seq_len} tokens"
+        self.drafted, self._parents, self._parents_dev, self._depth_rows = 0, None, None, None
+        self.seq_len = int(length)
+        self.pooled_chunks = min(self.pooled_chunks, self.seq_len // self.S)
+        self.has_prior = self.has_prior and self.pooled_chunks > 0
+        self._keep_pages(self.seq_len)
+
+    def free(self):
+        """Give up every token: all pages are free."""
+        self.truncate(0)
+
+    def fork(self, source):
+        """Sequence b goes on from where sequence ``source[b]`` is (B ints; parallel samples, beams).  Pages are shared; a
+        partly filled one is copied when one of its users writes on it."""
+        assert not self.drafted, "tokens are on trial: accept() first"
+        source = [int(s) for s in source]
+        if len(source) != self.B or any(not 0 <= s < self.B for s in source):
+            raise ValueError(f"fork: {source} are not {self.B} sequences")
+        who = [b for b, s in enumerate(source) if s != b]
+        if not who:
+            return
+        pages = [list(self._pages[s]) for s in source]
+        for b in who:
+            for page in pages[b]:
+                self._users[page] += 1
+        for b in who:
+            self._give_back(self._pages[b])
+        self._pages = pages
+        dev = self.page_table.device
+        to, fr = torch.tensor(who, device=dev), torch.tensor([source[b] for b in who], device=dev)
+        self.page_table[to] = self.page_table[fr]
+        n = self.pooled_chunks
+        self.lmk_hm[to, :, :n] = self.lmk_hm[fr, :, :n]
+        if self.prior_hm is not None:
+            self.prior_hm[to, :, :n] = self.prior_hm[fr, :, :n]
+
+    def compact(self):
+        """Move the pages in use to the front of the pools; returns their number (the pools behind it are free)."""
+        used = [p for p in range(self.num_pages) if self._users[p]]
+        n = len(used)
+        holes = [p for p in range(n) if not self._users[p]]
+        moved = dict(zip([p for p in used if p >= n], holes))
+        if moved:
+            copy_pages(self._pools(), list(moved.keys()), list(moved.values()))
+            for old, new in moved.items():
+                self._users[new], self._users[old] = self._users[old], 0
+            self._pages = [[moved.get(p, p) for p in pages] for pages in self._pages]
+            self.free_pages = list(range(self.num_pages - 1, n - 1, -1))
+            mapped = max(len(p) for p in self._pages)
+            self.page_table[:, :mapped] = torch.tensor(self._pages, dtype=torch.int32, device=self.page_table.device)
+        return n
 
     def gather_contiguous(self):
         """(B, seq_len, H, D) keys and values in token order (for the local branch, or checks)."""
@@ -331,19 +531,57 @@ class HiLSPagedLayer:
         v = self.v_pages[pg].permute(0, 1, 3, 2, 4).reshape(self.B, n * S, self.H, self.D)[:, : self.seq_len]
         return k.contiguous(), v.contiguous()
 
+    def local_attend(self, q, window_size, mask_lmk=True, expand_to_chunk=True, sm_scale=None):
+        """The local branch for the last ``q.shape[1]`` positions straight on the pages, or for the drafted tokens, each
+        with its own ancestors: (o (B,T,h_q,D), lse (B,T,h_q)) for ``hils_attend`` and the merge."""
+        assert not self.drafted or q.shape[1] == self.drafted, f"{self.drafted} tokens are on trial, got {q.shape[1]} queries"
+        return paged_flex_attn(q, self.k_pages, self.v_pages, self.page_table, self.seq_len + self.drafted, window_size,
+                               parents=self._parents_dev, mask_lmk=mask_lmk, expand_to_chunk=expand_to_chunk,
+                               sm_scale=sm_scale)
+
     def hils_attend(self, q, lse_swa, topk, window_size, sm_scale=None, _debug=None, dense_keys=True):
-        """The remote branch for the last ``q.shape[1]`` positions: selection, inter-chunk softmax (with
-        the prior bias once ``update`` has been given prior queries) and sparse attention straight on
-        the pages.  ``dense_keys``: stream the per-sequence head-major chunk keys (default) instead of
-        the per-page ones.  Returns (o (B,Lq,h_q,D), weights (B,Lq,h_q,topk+1), indices (B,Lq,H,topk)
+        """The remote branch for the last ``q.shape[1]`` positions (or for the drafted tokens, at the positions of their
+        depths): selection, inter-chunk softmax (with the prior bias once ``update`` has been given prior queries) and
+        sparse attention straight on the pages.  ``dense_keys``: stream the per-sequence head-major chunk keys (default)
+        instead of the per-page ones.  Returns (o (B,Lq,h_q,D), weights (B,Lq,h_q,topk+1), indices (B,Lq,H,topk)
         as chunk numbers of the sequence)."""
+        if self.drafted:
+            return self._drafts_attend(q, lse_swa, topk, window_size, sm_scale, dense_keys)
+        return self._attend(q, lse_swa, self.seq_len, topk, window_size, sm_scale, _debug, dense_keys)
+
+    def _attend(self, q, lse_swa, seq_len, topk, window_size, sm_scale, _debug, dense_keys):
         if dense_keys:
-            return paged_hils_attend(q, self.k_pages, self.v_pages, None, self.page_table, lse_swa, self.seq_len,
+            return paged_hils_attend(q, self.k_pages, self.v_pages, None, self.page_table, lse_swa, seq_len,
                                      topk, window_size, sm_scale=sm_scale, _debug=_debug, lmk_dense=self.lmk_hm,
                                      prior_dense=self.prior_hm if self.has_prior else None)
         return paged_hils_attend(q, self.k_pages, self.v_pages, self.lmk_pages, self.page_table, lse_swa,
-                                 self.seq_len, topk, window_size, sm_scale=sm_scale, _debug=_debug,
+                                 seq_len, topk, window_size, sm_scale=sm_scale, _debug=_debug,
                                  prior_pages=self.prior_pages if self.has_prior else None)
+
+    def _drafts_attend(self, q, lse_swa, topk, window_size, sm_scale, dense_keys):
+        """A token at position p selects among the chunks before floor((p - window + 1) / 64): tokens with the same limit
+        go through one call, up to 64 of them at positions whose limit with a window of 1 is that one."""
+        S, T = self.S, self.drafted
+        assert q.shape[1] == T, f"{T} tokens are on trial, got {q.shape[1]} queries"
+        back = window_size - 1 if window_size > 0 else 0
+        limits = [[max(self.seq_len + d - back, 0) // S for d in row] for row in self._depth_rows]
+        if max(max(row) for row in limits) > self.pooled_chunks:
+            raise ValueError(f"drafted tokens are too deep for a window of {window_size}: the remote branch cannot select "
+                             "drafted chunks")
+        out = None
+        for limit in sorted({x for row in limits for x in row}):
+            parts = []
+            for t0 in range(0, T, S):
+                t1 = min(t0 + S, T)
+                parts.append(self._attend(q[:, t0:t1], lse_swa[:, t0:t1], max(S, limit * S + t1 - t0), topk, 1, sm_scale,
+                                          None, dense_keys))
+            got = [p[0] if len(parts) == 1 else torch.cat(p, 1) for p in zip(*parts)]
+            if out is None:
+                out = got  # (the others replace theirs)
+                continue
+            mine = torch.tensor([[x == limit for x in row] for row in limits], device=q.device).view(-1, T, 1, 1)
+            out = [torch.where(mine, g, o) for g, o in zip(got, out)]
+        return tuple(out)
 
 
 def paged_hils_attend(q, k_pages, v_pages, lmk_pages, page_table, lse_swa, seq_len, topk, window_size,
