@@ -10,7 +10,7 @@
 // A row is a (token, query head of the KV head's group) pair.  Two kernels, both with the rows as the columns of the matrix
 // products S^T = K q^T and O^T += V^T P (a row's scores, maximum and sum stay in the lanes that hold its column):
 //   paged_attn_rows   16 or 32 rows a workgroup, its wavefronts share the keys (bound by the memory system),
-//   paged_attn_tiles  128 rows a workgroup, 32 a wavefront, pages staged in LDS (bound by the matrix and vector units).
+//   paged_attn_tiles  64, 128 or 256 rows a workgroup, 32 a wavefront, pages staged in LDS (bound by the matrix and vector units).
 // A long range of keys is split over workgroups; paged_attn_join adds their shares up, in a fixed order.
 // Scores, maxima, sums and outputs are fp32; probabilities are rounded to bf16 for the second product (half a step of
 // 2^-9 each, of random sign, about the size of the output's own rounding), their sum is taken before the rounding.
@@ -19,6 +19,7 @@
 // behind the last token, a rejected draft) would turn into a NaN.  A row whose result is no finite number is therefore
 // computed once more, token by token over the slots that it sees alone (paged_redo_row): the common call pays a comparison.
 #include "common.h"
+#include "lds_dma.h"
 #include "../../include/hils_amd.h"
 
 #define PA_PAGE 64
@@ -43,6 +44,23 @@ struct PagedSpan {
   int base, lo, hi, p0, p1;  // committed tokens, first slot and end of what any row sees, pages of this workgroup's share
   bool alive;
 };
+
+// What a workgroup works on.  The row blocks of a (sequence, KV head, share) read the same pages: neighbours on one XCD (the
+// hardware hands consecutive workgroups to the eight XCDs in turn).  False for the padding at the end.
+struct PagedUnit {
+  int blk, share, hk, b;
+};
+__device__ __forceinline__ bool paged_unit(const PagedDims& dm, PagedUnit& u) {
+  const int total = dm.n_blk * dm.n_split * dm.H * dm.B, per_xcd = (total + 7) / 8;
+  const int id = (int)(blockIdx.x % 8) * per_xcd + (int)(blockIdx.x / 8);
+  if (id >= total) return false;
+  const int rest = id / dm.n_blk, pair = rest / dm.n_split;
+  u.blk = id - rest * dm.n_blk;
+  u.share = rest - pair * dm.n_split;
+  u.b = pair / dm.H;
+  u.hk = pair - u.b * dm.H;
+  return true;
+}
 
 __device__ __forceinline__ int paged_left(int p, const PagedDims& dm) {
   const int left = p - dm.window + 1;
@@ -72,13 +90,22 @@ __device__ __forceinline__ PagedSpan paged_span(const PagedDims& dm, int b, int 
 
 // Ancestors of the tokens t0 .. t0 + nt - 1 as bits of slots base + u, and the first committed slot each sees.  A token whose
 // way to the root passes a parent that is neither -1 nor an earlier token takes no part: it sees nothing.
+// par: this thread's parents as paged_parents() read them (before loads that are not to be waited for here).
 // par_s: T words, mask_s: nt rows of PA_WORDS, left_s: nt words.  Ends without a barrier.
-__device__ __forceinline__ void paged_tree(const PagedDims& dm, int b, int base, int t0, int nt, int tid, int n_thr, int* par_s,
-                                           unsigned* mask_s, int* left_s) {
-  const int32_t* par = dm.parents + (long)b * dm.parents_stride;
-  for (int i = tid; i < dm.T; i += n_thr) par_s[i] = par[i];
-  for (int i = tid; i < nt * PA_WORDS; i += n_thr) mask_s[i] = 0;
-  __syncthreads();
+template <int NT>
+__device__ __forceinline__ void paged_parents(const PagedDims& dm, int b, int tid, int (&par)[(PA_MAX_TREE + NT - 1) / NT]) {
+  const int32_t* from = dm.parents + (long)b * dm.parents_stride;
+#pragma unroll
+  for (int i = 0; i < (PA_MAX_TREE + NT - 1) / NT; ++i) par[i] = tid + i * NT < dm.T ? from[tid + i * NT] : -2;
+}
+template <int NT>
+__device__ __forceinline__ void paged_tree(const PagedDims& dm, int base, int t0, int nt, int tid,
+                                           const int (&par)[(PA_MAX_TREE + NT - 1) / NT], int* par_s, unsigned* mask_s, int* left_s) {
+#pragma unroll
+  for (int i = 0; i < (PA_MAX_TREE + NT - 1) / NT; ++i)
+    if (tid + i * NT < dm.T) par_s[tid + i * NT] = par[i];
+  for (int i = tid; i < nt * PA_WORDS; i += NT) mask_s[i] = 0;
+  lds_barrier();
   if (tid >= nt || t0 + tid >= dm.T) {
     if (tid < nt) left_s[tid] = 0x7fffffff;
     return;
@@ -236,7 +263,9 @@ paged_attn_rows(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, cons
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, j = lane >> 4;
-  const int blk = blockIdx.x / dm.n_split, share = blockIdx.x % dm.n_split, hk = blockIdx.y, b = blockIdx.z;
+  PagedUnit at;
+  if (!paged_unit(dm, at)) return;
+  const int blk = at.blk, share = at.share, hk = at.hk, b = at.b;
   const int n_rows = dm.T * dm.G, r0 = blk * ROWS;
   const int r1 = r0 + ROWS < n_rows ? r0 + ROWS : n_rows;
   const PagedSpan sp = paged_span(dm, b, r0, r1, share);
@@ -251,6 +280,8 @@ paged_attn_rows(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, cons
     pages_of = u < u1 ? table[u >> 1] : -1;
   };
   ask_pages(u0 + wave);
+  int par[TREE ? (PA_MAX_TREE + NWV * 64 - 1) / (NWV * 64) : 1];
+  if constexpr (TREE) paged_parents<NWV * 64>(dm, b, tid, par);
   bf16x8_t qb[NR][KS];
   int row_t[NR];
 #pragma unroll
@@ -379,9 +410,9 @@ paged_attn_rows(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, cons
     auto page_at = [&](int i) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(pages_of, i & 63); };
     int pg_a = page_at(0), pg_c;
     if (n_mine > 0) issue(ka, va, pg_a, (u0 + wave) & 1);
-    if (TREE) paged_tree(dm, b, sp.base, t0, ROWS, tid, NWV * 64, par_s, mask_s, left_s);
+    if constexpr (TREE) paged_tree<NWV * 64>(dm, sp.base, t0, ROWS, tid, par, par_s, mask_s, left_s);
     if (tid == 0) odd_s = 0;
-    __syncthreads();
+    lds_barrier();
 #pragma unroll
     for (int rt = 0; rt < NR; ++rt) {
       const bool live = row_t[rt] >= 0 && sp.alive;
@@ -400,7 +431,10 @@ paged_attn_rows(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, cons
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qb[rt][ks]));
     auto next_page = [&](int i) __attribute__((always_inline)) {  // page of this wavefront's unit i, asked for 64 at a time
-      if ((i & 63) == 0) ask_pages(u0 + wave + i * NWV);
+      if ((i & 63) == 0) {
+        ask_pages(u0 + wave + i * NWV);
+        asm volatile("" : "+v"(pages_of));  // (waited for here: behind the branch, every unit would wait for all loads)
+      }
       return page_at(i);
     };
     int u = u0 + wave, i = 0;
@@ -466,312 +500,405 @@ paged_attn_rows(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, cons
 }
 
 // ---- many rows ---------------------------------------------------------------------------------
-// 32 rows a wavefront, four wavefronts; a page's keys and values go through registers into one of two LDS buffers while the
-// page before is worked on.  Both row-major, 16-byte piece p of row r at p ^ (r & pieces - 1), which no read conflicts over.
-template <int D>
-static constexpr size_t paged_tiles_smem() { return 2 * 2 * (size_t)PA_PAGE * 2 * D; }
+// 32 rows a wavefront; pages go straight into LDS, keys into one of four buffers, values into one of four others, asked for
+// three steps before they are used.  32x32x16 products: a row's scores of half a page (32 tokens) are 16 registers of two
+// lanes, which are the second product's operand as they are.  A step issues, half by half, the products of page p's output
+// and of page p + 1's scores between the exponentials of the half page behind (the matrix and vector instructions of one
+// wavefront overlap, those of two that run in step hardly do).  The exponentials' reference point follows a row's maximum
+// only when a score is more than 2^6 above it: the others need no reduction over lanes and no rescaling, and probabilities
+// of up to 2^6 enter sum and output alike.
+// The buffers come first: their places are then plain offsets, and a buffer's number is two bits of them.
+template <int D, int NW, bool TREE>
+static constexpr size_t paged_tiles_smem() {
+  return 2 * 4 * (size_t)PA_PAGE * 2 * D + (TREE ? (NW * 32 * (PA_WORDS + 1) + PA_MAX_TREE) * sizeof(int) : 0);
+}
 
-template <int D, bool TREE>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))
+template <int D, int NW, bool TREE>
+__global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)))
 paged_attn_tiles(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, const bf16_t* __restrict__ v, PagedDims dm,
                  PagedOut out) {
-  constexpr int RT = 2, NT = 256, ROWS = 128, KS = D / 32, DT = D / 16, RP = 2 * D, SEG = D / 8;
-  constexpr int PT = 64 * SEG / NT;        // 16-byte pieces per thread of a page's keys (and of its values)
-  constexpr int TILE = PA_PAGE * RP;       // bytes of a page's keys
-  constexpr float LAZY = 6.f;              // log2 of the growth of a row's maximum that moves its reference point
+  constexpr int NT = NW * 64, ROWS = NW * 32, KS = D / 16, FT = D / 32, RP = 2 * D, SEG = D / 8;
+  constexpr int NB = 4, PAGE = PA_PAGE * RP, NP = PAGE / 1024 / NW;  // loads of a page's keys per wavefront
+  static_assert(NP >= 1 && NP * NW * 1024 == PAGE, "every wavefront loads whole rows");
+  constexpr float LAZY = 6.f;
   extern __shared__ __align__(16) unsigned char pa_dyn[];
-  __shared__ int par_s[TREE ? PA_MAX_TREE : 1], left_s[ROWS];
-  __shared__ unsigned mask_s[TREE ? ROWS * PA_WORDS : 1];
+  unsigned* const mask_s = (unsigned*)(pa_dyn + 2 * NB * PAGE);
+  int* const left_s = (int*)(mask_s + ROWS * PA_WORDS);
+  int* const par_s = left_s + ROWS;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int col = lane & 15, j = lane >> 4;
-  // the row blocks of a (sequence, KV head, share) read the same pages: neighbours on one XCD
-  const int total = dm.n_blk * dm.n_split * dm.H * dm.B, per_xcd = (total + 7) / 8;
-  const int id = (int)(blockIdx.x % 8) * per_xcd + (int)(blockIdx.x / 8);
-  if (id >= total) return;
-  const int blk = id % dm.n_blk, share = id / dm.n_blk % dm.n_split, pair = id / dm.n_blk / dm.n_split;
-  const int hk = pair % dm.H, b = pair / dm.H;
+  const int col = lane & 31, h = lane >> 5;
+  PagedUnit at;
+  if (!paged_unit(dm, at)) return;
+  const int blk = at.blk, share = at.share, hk = at.hk, b = at.b;
   const int n_rows = dm.T * dm.G, r0 = blk * ROWS;
   const int r1 = r0 + ROWS < n_rows ? r0 + ROWS : n_rows;
   const PagedSpan sp = paged_span(dm, b, r0, r1, share);
   const int32_t* table = dm.table + (long)b * dm.max_pages;
   const int t0 = hils_udiv(r0, dm.G, dm.g_magic);
-  const long page_el = (long)dm.H * PA_PAGE * D, head_el = (long)hk * PA_PAGE * D;
 
-  int pages_of = -1;
-  auto ask_pages = [&](int first) __attribute__((always_inline)) {
-    pages_of = first + lane < sp.p1 ? table[first + lane] : -1;
+  const int p0 = __builtin_amdgcn_readfirstlane(sp.p0);
+  const int n = __builtin_amdgcn_readfirstlane(sp.p1 - sp.p0);
+  int pages_of = -1, pages_at = p0;  // lane i holds the page of chunk pages_at + i
+  auto ask_pages = [&]() __attribute__((always_inline)) {
+    pages_of = pages_at + lane < sp.p1 ? table[pages_at + lane] : -1;
   };
-  auto page_at = [&](int p) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(pages_of, (p - sp.p0) & 63); };
-  pa_u4 kd[PT], vd[PT];
-  auto issue = [&](int page) __attribute__((always_inline)) {
-    const long at = ((unsigned)page < (unsigned)dm.num_pages ? page * page_el : 0) + head_el + tid * 8;
-#pragma unroll
-    for (int i = 0; i < PT; ++i) kd[i] = *(const pa_u4*)(k + at + i * NT * 8);
-#pragma unroll
-    for (int i = 0; i < PT; ++i) vd[i] = *(const pa_u4*)(v + at + i * NT * 8);
-  };
-  auto put = [&](int buf) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < PT; ++i) {
-      const int pc = tid + NT * i, row = pc / SEG;
-      unsigned char* to = pa_dyn + buf * 2 * TILE + row * RP + ((pc % SEG) ^ (row & (SEG - 1))) * 16;
-      *(pa_u4*)to = kd[i];
-      *(pa_u4*)(to + TILE) = vd[i];
+  auto page_at = [&](int p) __attribute__((always_inline)) {
+    if (p - pages_at >= 64) {
+      pages_at += 64;
+      ask_pages();
+      asm volatile("" : "+v"(pages_of));  // (waited for here: behind the branch, every step would wait for all its loads)
     }
+    return __builtin_amdgcn_readlane(pages_of, p - pages_at);
   };
-  ask_pages(sp.p0);
-  int page = page_at(sp.p0);
-  if (sp.p0 < sp.p1) issue(page);
-
-  bf16x8_t qa[RT][KS];
-  int row_t[RT];
+  unsigned d_off[NP < 4 ? NP : 4];  // (the fifth load's places are the first one's, 4 KiB further)
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    const int r = r0 + wave * 32 + rt * 16 + col;
-    const int rc = r < r1 ? r : r1 - 1;
-    const int t = hils_udiv(rc, dm.G, dm.g_magic), g = rc - t * dm.G;
-    row_t[rt] = r < r1 ? t : -1;
-    const bf16_t* qp = q + b * dm.q_sb + t * dm.q_st + (hk * dm.G + g) * dm.q_sh + j * 8;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) qa[rt][ks] = *(const bf16x8_t*)(qp + ks * 32);
+  for (int i = 0; i < (NP < 4 ? NP : 4); ++i) {
+    const int x = (wave * NP + i) * 64 + lane, row = x / SEG, pc = x % SEG;
+    d_off[i] = (unsigned)(row * RP + (pc ^ lz_swz<D>(row)) * 16);
   }
-  if (TREE) paged_tree(dm, b, sp.base, t0, ROWS, tid, NT, par_s, mask_s, left_s);
-  if (sp.p0 < sp.p1) put(0);
-  __syncthreads();
-  int vlo[RT];
-  unsigned vspan[RT];
-  const unsigned* mrow[RT];
-  int some_lo = 0x7fffffff, all_lo = 0, some_hi = 0, all_hi = 0x7fffffff;  // slots that any row sees, that all see
+  const unsigned lds0 = __builtin_amdgcn_readfirstlane(lz_lds_addr(pa_dyn) + wave * (NP * 1024));
+  const unsigned long long head_b = (unsigned long long)hk * PAGE, page_b = (unsigned long long)dm.H * PAGE;
+  // Page x's keys lie in buffer gray(x % 4), its values in that buffer of the four behind: from one page to the next one bit
+  // of the buffer's number changes, the lower and the higher in turn.
+  unsigned known = 0;  // bit i: the page i fetches back is mapped
+  auto k_buffer = [&](int x) __attribute__((always_inline)) { return lds0 + (unsigned)((x & 3) ^ (x >> 1 & 1)) * PAGE; };
+  auto v_buffer = [&](int x) __attribute__((always_inline)) { return k_buffer(x) + NB * PAGE; };
+  auto page_place = [&](int x) __attribute__((always_inline)) {  // where in the pools page x lies (past the end: anywhere)
+    const int page = x < n ? page_at(p0 + x) : -1;
+    const bool mapped = (unsigned)page < (unsigned)dm.num_pages;
+    known = known << 1 | (unsigned)mapped;
+    return lz_uniform((mapped ? page * page_b : 0) + head_b);
+  };
+  const unsigned long long k_pool = lz_uniform((unsigned long long)k), v_pool = lz_uniform((unsigned long long)v);
+  auto fetch = [&](unsigned long long from, unsigned to) __attribute__((always_inline)) {
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    const bool live = row_t[rt] >= 0 && sp.alive;
-    const int i = live ? row_t[rt] - t0 : 0;
-    int lo = TREE ? left_s[i] : paged_left(sp.base + row_t[rt], dm);
+    for (int i = 0; i < NP; ++i) lz_dma16(to + i * 1024, d_off[i & 3], from + (i >> 2) * 4096);
+  };
+
+  const int r = r0 + wave * 32 + col;
+  const int rc = r < r1 ? r : r1 - 1;
+  const int my_t = hils_udiv(rc, dm.G, dm.g_magic), my_g = rc - my_t * dm.G;
+  const bool live = r < r1 && sp.alive;
+  bf16x8_t qa[KS];
+  {
+    const bf16_t* qp = q + b * dm.q_sb + my_t * dm.q_st + (hk * dm.G + my_g) * dm.q_sh + h * 8;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qa[ks] = *(const bf16x8_t*)(qp + ks * 16);
+  }
+  int par[TREE ? (PA_MAX_TREE + NT - 1) / NT : 1];
+  if constexpr (TREE) paged_parents<NT>(dm, b, tid, par);
+  ask_pages();
+  // (the queries and pages are here from now on: the compiler's waits know nothing of the loads into LDS and would wait for
+  // them too)
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qa[ks]));
+  asm volatile("" : "+v"(pages_of));
+  if constexpr (TREE) asm volatile("" : "+v"(par[0]), "+v"(par[(PA_MAX_TREE - 1) / NT]));
+  const unsigned long long place0 = page_place(0), place1 = page_place(1), place2 = page_place(2);
+  unsigned long long place = page_place(3);  // of page x + 3 before step x
+  if (n > 0) {
+    fetch(k_pool + place0, k_buffer(0));
+    fetch(k_pool + place1, k_buffer(1));
+    fetch(v_pool + place0, v_buffer(0));
+  }
+  if constexpr (TREE) paged_tree<NT>(dm, sp.base, t0, ROWS, tid, par, par_s, mask_s, left_s);
+  if (n > 0) {
+    fetch(k_pool + place2, k_buffer(2));
+    fetch(v_pool + place1, v_buffer(1));
+    fetch(k_pool + place, k_buffer(3));
+    fetch(v_pool + place2, v_buffer(2));
+  }
+  if constexpr (TREE) lds_barrier();
+  // visible slots of the row: [vlo, vlo + vspan], and in a tree the mask's bits behind the committed tokens
+  int vlo;
+  unsigned vspan;
+  int all_lo = 0, all_hi = 0x7fffffff;  // slots that all rows of the wavefront see
+  const unsigned* mrow = TREE ? mask_s + (live ? my_t - t0 : 0) * PA_WORDS : nullptr;
+  {
+    int lo = TREE ? left_s[live ? my_t - t0 : 0] : paged_left(sp.base + my_t, dm);
     lo = lo > 0 ? lo : 0;
-    const int last = TREE ? sp.base - 1 : sp.base + row_t[rt];
+    const int last = TREE ? sp.base - 1 : sp.base + my_t;
     const bool some = live && last >= lo;
-    vlo[rt] = some ? lo : 0x7fffffff;
-    vspan[rt] = some ? (unsigned)(last - lo) : 0u;
-    if (TREE) mrow[rt] = mask_s + i * PA_WORDS;
-    if (live) {  // (a drafted token sees itself at least, one that takes no part has its window's start out of reach)
-      const int from = TREE && lo < 0x7fffffff && lo > sp.base ? sp.base : lo, to = TREE ? sp.base + dm.T : last + 1;
-      some_lo = from < some_lo ? from : some_lo;
-      all_lo = lo > all_lo ? lo : all_lo;
-      some_hi = to > some_hi ? to : some_hi;
-      all_hi = last + 1 < all_hi ? last + 1 : all_hi;
+    vlo = some ? lo : 0x7fffffff;
+    vspan = some ? (unsigned)(last - lo) : 0u;
+    if (live) {
+      all_lo = lo;
+      all_hi = last + 1;
     }
   }
 #pragma unroll
-  for (int x = 1; x < 16; x <<= 1) {
-    some_lo = min(some_lo, __shfl_xor(some_lo, x, 64));
+  for (int x = 1; x < 32; x <<= 1) {
     all_lo = max(all_lo, __shfl_xor(all_lo, x, 64));
-    some_hi = max(some_hi, __shfl_xor(some_hi, x, 64));
     all_hi = min(all_hi, __shfl_xor(all_hi, x, 64));
   }
-  some_lo = __builtin_amdgcn_readfirstlane(some_lo);
   all_lo = __builtin_amdgcn_readfirstlane(all_lo);
-  some_hi = __builtin_amdgcn_readfirstlane(some_hi);
   all_hi = __builtin_amdgcn_readfirstlane(all_hi);
 
-  f32x4_t acc[RT][DT];
-  float m_run[RT], l_run[RT];  // reference point (score units) and sum, per row (lane & 15)
+  f32x16_t acc[FT];
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
+  for (int ft = 0; ft < FT; ++ft)
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) acc[rt][dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    m_run[rt] = HILS_NEG_INF;
-    l_run[rt] = 0.f;
-  }
-  unsigned k_off[KS], v_off[DT];
+    for (int i = 0; i < 16; ++i) acc[ft][i] = 0.f;
+  float ref = HILS_NEG_INF, l_run = 0.f;  // reference point (log2 units) and this lane's share of the sum
+  unsigned k_off[KS], v_off[FT][2];       // this lane's places in a half page, in the buffers of this step
 #pragma unroll
-  for (int ks = 0; ks < KS; ++ks) k_off[ks] = (unsigned)(col * RP + ((ks * 4 + j) ^ (col & (SEG - 1))) * 16);
+  for (int ks = 0; ks < KS; ++ks) k_off[ks] = (unsigned)(col * RP + ((2 * ks + h) ^ lz_swz<D>(col)) * 16);
 #pragma unroll
-  for (int dt = 0; dt < DT; ++dt) {
-    const int row = 4 * j + (col >> 2);
-    v_off[dt] = (unsigned)(row * RP + ((dt * 2 + (col >> 1 & 1)) ^ (row & (SEG - 1))) * 16 + (col & 1) * 8);
-  }
+  for (int ft = 0; ft < FT; ++ft)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int row = 4 * h + 8 * e + ((lane & 15) >> 2), pc = ft * 4 + (lane >> 4 & 1) * 2 + (lane >> 1 & 1);
+      v_off[ft][e] = (unsigned)(NB * PAGE + row * RP + (pc ^ lz_swz<D>(row)) * 16 + (lane & 1) * 8);
+    }
 
-  // (the queries are here from now on: waited for inside the loop, the page under way would be waited for with them)
+  auto products = [&](f32x16_t& st, int half) __attribute__((always_inline)) {
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt)
+    for (int i = 0; i < 16; ++i) st[i] = 0.f;
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qa[rt][ks]));
-
-  auto tile_step = [&](int p, const unsigned char* k_s) __attribute__((always_inline)) {
-    const unsigned char* v_s = k_s + TILE;
-    f32x4_t s[RT][4];  // scores, then probabilities: slot tt*16 + 4j + i of the page, row lane & 15
-    float corr[RT];
-    bool rescale = false;
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-      for (int tt = 0; tt < 4; ++tt) s[rt][tt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int tt = 0; tt < 4; ++tt)
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        const bf16x8_t a = *(const bf16x8_t*)(k_s + k_off[ks] + tt * 16 * RP);
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) s[rt][tt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, qa[rt][ks], s[rt][tt], 0, 0, 0);
-        if (ks == KS - 1 && (tt & 1)) __builtin_amdgcn_sched_barrier(0);  // (operand reads of later steps stay behind)
-      }
-    if (p * PA_PAGE < all_lo || p * PA_PAGE + PA_PAGE > all_hi) {  // some row does not see all of the page
-      const int slot0 = p * PA_PAGE + 4 * j;
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        const unsigned from = (unsigned)(slot0 - vlo[rt]);
-        uint64_t extra = 0;
-        if (TREE && p * PA_PAGE + PA_PAGE > sp.base) {
-          const int off = p * PA_PAGE - sp.base;
-          const unsigned x0 = off > -32 && off < dm.T ? paged_bits(mrow[rt], off) : 0u;
-          const unsigned x1 = off + 32 < dm.T ? paged_bits(mrow[rt], off + 32) : 0u;
-          extra = ((uint64_t)x1 << 32 | x0) >> (4 * j);
+    for (int ks = 0; ks < KS; ++ks)
+      st = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8_t*)(pa_dyn + (k_off[ks] + half * 32 * RP)), qa[ks], st, 0, 0, 0);
+  };
+  // scores of a half of page x: -inf where the row does not see a token (token (i >> 2) * 8 + 4 h + (i & 3) in register i)
+  auto hide = [&](f32x16_t& st, int x, int half, int back) __attribute__((always_inline)) {  // back: fetches of keys since
+    const int first = (p0 + x) * PA_PAGE + half * 32;
+    const bool mapped = known >> back & 1;
+    if (first < all_lo || first + 32 > all_hi || !mapped) {
+      unsigned seen = 0;  // bit i: the row sees token first + i
+      if (mapped) {
+        const int lo = vlo - first, hi = (int)((unsigned)vlo + vspan - (unsigned)first);
+        if (lo < 32 && hi >= 0) seen = ~0u << (lo > 0 ? lo : 0) & ~0u >> (hi < 31 ? 31 - hi : 0);
+        if (TREE) {
+          if (dm.mask_lmk && half) seen &= 0x7fffffffu;
+          const int off = first - sp.base;
+          if (off > -32 && off < dm.T) seen |= paged_bits(mrow, off);
         }
-#pragma unroll
-        for (int tt = 0; tt < 4; ++tt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            bool see = from + (unsigned)(tt * 16 + i) <= vspan[rt];
-            if (TREE && dm.mask_lmk && tt == 3 && i == 3) see = see && j != 3;
-            if (TREE) see = see || (extra >> (tt * 16 + i) & 1);
-            s[rt][tt][i] = see ? s[rt][tt][i] : HILS_NEG_INF;
-          }
       }
+      seen >>= 4 * h;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) st[i] = seen >> ((i >> 2) * 8 + (i & 3)) & 1 ? st[i] : HILS_NEG_INF;
     }
     // a committed landmark is its page's last token (a drafted one has been left out of the masks)
-    if (dm.mask_lmk && (!TREE || p * PA_PAGE + PA_PAGE <= sp.base)) {
+    if (half && dm.mask_lmk && (!TREE || first + 32 <= sp.base)) st[15] = h == 1 ? HILS_NEG_INF : st[15];
+  };
+  // Probabilities e[i0 .. i0 + N) of scores about the reference point, into the sums and, in pairs, into the second product's
+  // operand.
+  float ref0 = 0.f;  // (the reference point, 0 where nothing has been seen)
+  auto weigh = [&](const f32x16_t& st, pa_u4 (&p)[2], float (&sum)[2], auto i0, auto count) __attribute__((always_inline)) {
+    constexpr int I0 = decltype(i0)::value, N = decltype(count)::value;
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) s[rt][3][3] = j == 3 ? HILS_NEG_INF : s[rt][3][3];
-    }
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      float mx = HILS_NEG_INF;
-#pragma unroll
-      for (int tt = 0; tt < 4; ++tt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[rt][tt][i]);
-      mx = rows_max(mx);
-      // the reference point of the exponentials follows the maximum only when that grows by more than 2^LAZY, or when
-      // nothing is accumulated yet: most pages rescale no accumulators
-      const bool fresh = l_run[rt] == 0.f;
-      const bool move = fresh | ((mx - m_run[rt]) * dm.c2 > LAZY);
-      const float m_new = move ? fmaxf(m_run[rt], mx) : m_run[rt];
-      const bool any = m_new > HILS_NEG_INF;
-      corr[rt] = (move & any & !fresh) ? __builtin_amdgcn_exp2f((m_run[rt] - m_new) * dm.c2) : 1.f;
-      const float mc = any ? m_new * dm.c2 : 0.f;
-      rescale |= corr[rt] != 1.f;
-      float sum = 0.f;
-#pragma unroll
-      for (int tt = 0; tt < 4; ++tt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float e = __builtin_amdgcn_exp2f(fmaf(s[rt][tt][i], dm.c2, -mc));  // masked: exp2(-inf) = 0
-          s[rt][tt][i] = e;
-          sum += e;
-        }
-      sum = rows_sum(sum);
-      l_run[rt] = l_run[rt] * corr[rt] + sum;
-      m_run[rt] = m_new;
-    }
-    if (__any(rescale)) {
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[rt][dt][i] *= corr[rt];
-    }
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      bf16x8_t pb[RT];
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        pa_u4 u;
-        u.x = pack_bf2(s[rt][2 * h][0], s[rt][2 * h][1]);
-        u.y = pack_bf2(s[rt][2 * h][2], s[rt][2 * h][3]);
-        u.z = pack_bf2(s[rt][2 * h + 1][0], s[rt][2 * h + 1][1]);
-        u.w = pack_bf2(s[rt][2 * h + 1][2], s[rt][2 * h + 1][3]);
-        pb[rt] = __builtin_bit_cast(bf16x8_t, u);
-      }
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) {
-        const unsigned char* at = v_s + v_off[dt] + (2 * h * 16) * RP;
-        const pa_s4 b0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) pa_s4*)at);
-        const pa_s4 b1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) pa_s4*)(at + 16 * RP));
-        const bf16x8_t a = __builtin_bit_cast(bf16x8_t, (pa_s8)__builtin_shufflevector(b0, b1, 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) acc[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, pb[rt], acc[rt][dt], 0, 0, 0);
-        if ((dt & 3) == 3) __builtin_amdgcn_sched_barrier(0);
-      }
+    for (int i = I0; i < I0 + N; i += 2) {
+      const float e0 = __builtin_amdgcn_exp2f(fmaf(st[i], dm.c2, -ref0)), e1 = __builtin_amdgcn_exp2f(fmaf(st[i + 1], dm.c2, -ref0));
+      sum[0] += e0;
+      sum[1] += e1;
+      p[i >> 3][i >> 1 & 3] = pack_bf2(e0, e1);
     }
   };
-
-  for (int p = sp.p0; p < sp.p1; ++p) {
-    const int now = page;
-    if (p + 1 < sp.p1) {
-      if (((p + 1 - sp.p0) & 63) == 0) ask_pages(p + 1);
-      page = page_at(p + 1);
-      issue(page);
+  typedef std::integral_constant<int, 0> Zero;
+  // The same for all 16 with the reference point moved to the maximum where a row has a score (mx: of this lane) far above it.
+  // Returns the factor that the accumulators are due.
+  auto settle = [&](const f32x16_t& st, pa_u4 (&p)[2], float mx) __attribute__((always_inline)) {
+    mx = lz_halves_max(mx) * dm.c2;
+    const float to = mx > ref + LAZY ? mx : ref;
+    const float corr = to > ref ? __builtin_amdgcn_exp2f(ref - to) : 1.f;  // exp2(-inf) = 0: nothing yet
+    ref = to;
+    ref0 = to > HILS_NEG_INF ? to : 0.f;
+    float sum[2] = {0.f, 0.f};
+    weigh(st, p, sum, Zero{}, std::integral_constant<int, 16>{});
+    l_run = fmaf(l_run, corr, sum[0] + sum[1]);
+    return corr;
+  };
+  auto highest = [](const f32x16_t& st) __attribute__((always_inline)) {
+    float mx = fmaxf(st[0], st[1]);
+#pragma unroll
+    for (int i = 2; i < 16; ++i) mx = fmaxf(mx, st[i]);
+    return mx;
+  };
+  f32x16_t sa, sb;  // scores of first halves, of second halves
+  pa_u4 pa[2], pb[2];
+  static_assert(NP <= KS, "half a step issues the loads of a page's keys or values");
+  constexpr int AH = 3;  // products of each kind that operands are read ahead of
+  // Step x: the products of page x's output and of page x + 1's scores, a pair of them at a time (D / 16 pairs a half), and
+  // between them the probabilities of the half page behind, from the scores that the half step before has left; the loads of
+  // page x + 3's values and x + 4's keys.
+  auto step = [&](int x, unsigned long long v_from, unsigned v_to, unsigned long long k_from, unsigned k_to) __attribute__((always_inline)) {
+    bf16x8_t va[AH + 1], ka[AH + 1];
+    auto operands = [&](int y) __attribute__((always_inline)) {
+      const int half = y / KS, s = y % KS / FT, ft = y % FT;
+      const unsigned char* a0p = pa_dyn + (v_off[ft][0] + (half * 32 + s * 16) * RP);
+      const unsigned char* a1p = pa_dyn + (v_off[ft][1] + (half * 32 + s * 16) * RP);
+      const pa_s4 a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) pa_s4*)a0p);
+      const pa_s4 a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) pa_s4*)a1p);
+      va[y % (AH + 1)] = __builtin_bit_cast(bf16x8_t, (pa_s8)__builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7));
+      ka[y % (AH + 1)] = *(const bf16x8_t*)(pa_dyn + (k_off[y % KS] + half * 32 * RP));
+    };
+    float sum[2], mx;
+    // the y-th pair; probabilities of `now` into pn
+    auto pair = [&](auto yc, f32x16_t& now, f32x16_t& nx, const pa_u4 (&p)[2], pa_u4 (&pn)[2]) __attribute__((always_inline)) {
+      constexpr int y = decltype(yc)::value, z = y % KS;
+      if constexpr (y + AH < 2 * KS) operands(y + AH);
+      acc[y % FT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va[y % (AH + 1)], __builtin_bit_cast(bf16x8_t, p[z / FT]), acc[y % FT], 0, 0, 0);
+      nx = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka[y % (AH + 1)], qa[z], nx, 0, 0, 0);
+      if constexpr (z < NP) lz_dma16((y < KS ? v_to : k_to) + z * 1024, d_off[z & 3], (y < KS ? v_from : k_from) + (z >> 2) * 4096);
+      if (z > 0) {  // (none beside the first pair: its scores are not there yet)
+        constexpr int per = KS == 8 ? 2 : 4, first = (z - 1) * per;
+        weigh(now, pn, sum, std::integral_constant<int, first>{}, std::integral_constant<int, z == KS - 1 ? 16 - first : per>{});
+        if (z == KS - 1) mx = highest(now);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    auto finish = [&](f32x16_t& now, pa_u4 (&pn)[2]) __attribute__((always_inline)) {
+      float l_new = l_run + (sum[0] + sum[1]);
+      asm volatile("" : "+v"(pn[0]), "+v"(pn[1]), "+v"(l_new), "+v"(mx));  // (taken between the products, not behind them)
+      __builtin_amdgcn_sched_barrier(0);
+      const bool moves = __any(mx * dm.c2 > ref + LAZY);
+      float corr = 1.f;
+      if (moves) corr = settle(now, pn, mx);
+      else l_run = l_new;
+      if (moves) {
+#pragma unroll
+        for (int ft = 0; ft < FT; ++ft)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[ft][i] *= corr;
+      }
+    };
+#define PA_PAIR(Y_, NOW_, NX_, P_, PN_) pair(std::integral_constant<int, Y_>{}, NOW_, NX_, P_, PN_)
+#define PA_HALF(Y_, NOW_, NX_, P_, PN_)                                                                             \
+  PA_PAIR(Y_ + 1, NOW_, NX_, P_, PN_);                                                                              \
+  PA_PAIR(Y_ + 2, NOW_, NX_, P_, PN_);                                                                              \
+  PA_PAIR(Y_ + 3, NOW_, NX_, P_, PN_);                                                                              \
+  if constexpr (KS == 8) {                                                                                          \
+    PA_PAIR(Y_ + 4, NOW_, NX_, P_, PN_);                                                                            \
+    PA_PAIR(Y_ + 5, NOW_, NX_, P_, PN_);                                                                            \
+    PA_PAIR(Y_ + 6, NOW_, NX_, P_, PN_);                                                                            \
+    PA_PAIR(Y_ + 7, NOW_, NX_, P_, PN_);                                                                            \
+  }
+#pragma unroll
+    for (int y = 0; y < AH; ++y) operands(y);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sa[i] = 0.f;
+    sum[0] = sum[1] = 0.f;
+    __builtin_amdgcn_sched_barrier(0);
+    PA_PAIR(0, sb, sa, pa, pb);
+    hide(sb, x, 1, 4);
+    asm volatile("" : "+v"(sb));  // (the exponentials stay behind this point, between the products)
+    __builtin_amdgcn_sched_barrier(0);
+    PA_HALF(0, sb, sa, pa, pb)
+    finish(sb, pb);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sb[i] = 0.f;
+    sum[0] = sum[1] = 0.f;
+    __builtin_amdgcn_sched_barrier(0);
+    PA_PAIR(KS, sa, sb, pb, pa);
+    hide(sa, x + 1, 0, 3);
+    asm volatile("" : "+v"(sa));
+    __builtin_amdgcn_sched_barrier(0);
+    PA_HALF(KS, sa, sb, pb, pa)
+    finish(sa, pa);
+#undef PA_HALF
+#undef PA_PAIR
+  };
+  if (n > 0) {
+    lz_landed<6 * NP>();  // keys of page 0
+    lds_barrier();
+    products(sa, 0);
+    products(sb, 1);
+    hide(sa, 0, 0, 3);
+    (void)settle(sa, pa, highest(sa));
+    for (int x = 0; x < n; ++x) {
+      lz_landed<4 * NP>();  // keys of x + 1, values of x
+      lds_barrier();        // ... of all wavefronts; keys of x and values of x - 1 have been read
+      const unsigned long long v_from = v_pool + place;
+      place = page_place(x + 4);
+      const unsigned other = x & 1 ? 2 * PAGE : PAGE;  // the bit in which the buffers of pages x and x + 1 differ
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) k_off[ks] ^= other;
+      step(x, v_from, v_buffer(x + 3), k_pool + place, k_buffer(x + 4));
+#pragma unroll
+      for (int ft = 0; ft < FT; ++ft)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) v_off[ft][e] ^= other;
     }
-    if ((unsigned)now < (unsigned)dm.num_pages && p * PA_PAGE < some_hi && p * PA_PAGE + PA_PAGE > some_lo)
-      tile_step(p, pa_dyn + ((p - sp.p0) & 1) * 2 * TILE);
-    if (p + 1 < sp.p1) put((p + 1 - sp.p0) & 1);
-    __syncthreads();
+    lz_landed<0>();
   }
 
+  // accumulator register i of tile ft is feature ft*32 + (i >> 2)*8 + 4h + (i & 3) of row `col`
+  const hils_uint2v two = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_run), __float_as_uint(l_run), false, false);
+  const float l = __uint_as_float(two.x) + __uint_as_float(two.y);
+  const float m = ref / dm.c2;  // (score units, as the joined shares have it)
+  const long row = ((long)b * dm.T + my_t) * dm.HQ + hk * dm.G + my_g;
+  float all = 0.f;
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    const int r = r0 + wave * 32 + rt * 16 + col;
-    const int rc = r < r1 ? r : r1 - 1;
-    const int t = hils_udiv(rc, dm.G, dm.g_magic), g = rc - t * dm.G;
-    const long row = ((long)b * dm.T + t) * dm.HQ + hk * dm.G + g;
-    float all = 0.f;
+  for (int ft = 0; ft < FT; ++ft)
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) all += (acc[rt][dt][0] + acc[rt][dt][1]) + (acc[rt][dt][2] + acc[rt][dt][3]);
-    if (r < r1) {
+    for (int i = 0; i < 16; ++i) all += acc[ft][i];
+  if (r < r1) {
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) paged_store4<D>(dm, out, row, share, dt * 4 + j, acc[rt][dt], m_run[rt], l_run[rt]);
-    }
-    uint64_t odd = __ballot(r < r1 && !(fabsf(all) < INFINITY));
-    odd = (odd | odd >> 16 | odd >> 32 | odd >> 48) & 0xffff;
-    if (odd) {
-      __builtin_amdgcn_s_waitcnt(0);  // (the stores above are in memory before the same wavefront writes there again)
-      while (odd) {
-        const int i = __builtin_ctzll(odd);
-        odd &= odd - 1;
-        const int rr = r0 + wave * 32 + rt * 16 + i, tr = hils_udiv(rr, dm.G, dm.g_magic), gr = rr - tr * dm.G;
-        const int left = TREE ? left_s[tr - t0] : paged_left(sp.base + tr, dm);
-        paged_redo_row<D>(dm, out, q + b * dm.q_sb + tr * dm.q_st + (hk * dm.G + gr) * dm.q_sh, k, v, table, hk, sp.base,
-                          sp.p0, sp.p1, tr, left, TREE ? mask_s + (tr - t0) * PA_WORDS : nullptr,
-                          ((long)b * dm.T + tr) * dm.HQ + hk * dm.G + gr, share, lane);
+    for (int ft = 0; ft < FT; ++ft)
+#pragma unroll
+      for (int i4 = 0; i4 < 4; ++i4) {
+        const f32x4_t x = {acc[ft][4 * i4], acc[ft][4 * i4 + 1], acc[ft][4 * i4 + 2], acc[ft][4 * i4 + 3]};
+        paged_store4<D>(dm, out, row, share, ft * 8 + i4 * 2 + h, x, m, l);
       }
+  }
+  uint64_t odd = __ballot(r < r1 && !(fabsf(all) < INFINITY));
+  odd = (odd | odd >> 32) & 0xffffffffu;
+  if (odd) {
+    __builtin_amdgcn_s_waitcnt(0);  // (the stores above are in memory before the same wavefront writes there again)
+    while (odd) {
+      const int i = __builtin_ctzll(odd);
+      odd &= odd - 1;
+      const int rr = r0 + wave * 32 + i, tr = hils_udiv(rr, dm.G, dm.g_magic), gr = rr - tr * dm.G;
+      const int left = TREE ? left_s[tr - t0] : paged_left(sp.base + tr, dm);
+      paged_redo_row<D>(dm, out, q + b * dm.q_sb + tr * dm.q_st + (hk * dm.G + gr) * dm.q_sh, k, v, table, hk, sp.base, sp.p0,
+                        sp.p1, tr, left, TREE ? mask_s + (tr - t0) * PA_WORDS : nullptr,
+                        ((long)b * dm.T + tr) * dm.HQ + hk * dm.G + gr, share, lane);
     }
   }
 }
 
 // ---- shares of a range added up ------------------------------------------------------------------
+// A wavefront a row: lane i weighs share i (there are up to 64), then groups of D / 4 lanes take every GR-th share, four loads
+// under way, and add up across the groups.
 template <int D>
 __global__ void __launch_bounds__(256) paged_attn_join(PagedOut out, int n_split, float c2) {
-  constexpr int LPR = D / 4;  // lanes per row, four features each
-  const long row = (long)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
-  const int d4 = threadIdx.x % LPR;
-  if (row >= out.n_rows) return;
+  constexpr int LPR = D / 4, GR = 64 / LPR;  // lanes per row of features, groups
+  const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, d4 = lane % LPR, gr = lane / LPR;
+  if (row >= out.n_rows) return;  // (a whole wavefront)
   const float* ml = out.part + out.n_rows * n_split * D + row * n_split * 2;
   const float* part = out.part + row * n_split * D + d4 * 4;
-  float M = HILS_NEG_INF;
-  for (int s = 0; s < n_split; ++s) M = fmaxf(M, ml[2 * s]);
-  float L = 0.f;
-  f32x4_t x = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < n_split; ++s) {
-    const float l = ml[2 * s + 1];
-    if (l == 0.f) continue;  // (nothing seen there)
-    const float f = M > HILS_NEG_INF ? __builtin_amdgcn_exp2f((ml[2 * s] - M) * c2) : 1.f;
-    const f32x4_t y = *(const f32x4_t*)(part + (long)s * D);
-    L = fmaf(f, l, L);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = fmaf(f, y[i], x[i]);
+  float m = HILS_NEG_INF, l = 0.f;
+  if (lane < n_split) {
+    m = ml[2 * lane];
+    l = ml[2 * lane + 1];
   }
+  const float M = wave_max(m);
+  // (a share that saw nothing counts for nothing, whatever lies there)
+  const float f = l == 0.f ? 0.f : M > HILS_NEG_INF ? __builtin_amdgcn_exp2f((m - M) * c2) : 1.f;
+  const float L = wave_sum(l == 0.f ? 0.f : f * l);
+  f32x4_t x = {0.f, 0.f, 0.f, 0.f};
+  for (int s0 = gr; s0 < n_split + gr; s0 += 4 * GR) {
+    f32x4_t y[4];
+    float w[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int s = s0 + u * GR;
+      w[u] = __shfl(f, s & 63, 64);
+      w[u] = s < n_split ? w[u] : 0.f;
+      y[u] = *(const f32x4_t*)(part + (long)(s < n_split ? s : 0) * D);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = w[u] != 0.f ? fmaf(w[u], y[u][i], x[i]) : x[i];
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (GR == 4) x[i] += __shfl_xor(x[i], 16, 64);
+    x[i] += __shfl_xor(x[i], 32, 64);
+  }
+  if (gr) return;
   const float inv = L == 0.f ? 0.f : 1.f / L;
   uint2 pk;
   pk.x = pack_bf2(x[0] * inv, x[1] * inv);
@@ -783,28 +910,60 @@ __global__ void __launch_bounds__(256) paged_attn_join(PagedOut out, int n_split
 // ---- host ----------------------------------------------------------------------------------------
 struct PagedPlan {
   bool tiles;
-  int nr, n_blk, n_split;
+  int nr, nw, n_blk, n_split;  // 16 nr rows a workgroup, or 32 nw
 };
 
 // Which kernel, and over how many workgroups a range of keys is split.
-static PagedPlan paged_plan(int B, int T, int HQ, int H, int window, int max_pages) {
-  PagedPlan pl;
-  const int rows = T * (HQ / H);
-  // pages of the longest range a workgroup can have
-  const long seen = (long)window + (T < 128 ? T : 128) + 2 * PA_PAGE - 3;
-  const int pages = (int)(seen / PA_PAGE < max_pages ? seen / PA_PAGE : max_pages);
-  pl.tiles = rows > 64 && (long)((rows + 31) / 32) * H * B * pages > 2048;
-  pl.nr = rows > 16 ? 2 : 1;
-  const int per = pl.tiles ? 128 : 16 * pl.nr;
-  pl.n_blk = (rows + per - 1) / per;
-  const long wgs = (long)pl.n_blk * H * B;
-  const long want = (2l * hils_device_cus() + wgs - 1) / wgs;  // two workgroups a compute unit
-  const int least = 8;                                         // pages of a share
-  int most = pages / least;
-  most = most > 1 ? most : 1;
-  pl.n_split = (int)(want < most ? want : most);
-  pl.n_split = pl.n_split > 64 ? 64 : pl.n_split;
-  return pl;
+// What the variants cost, in microseconds, from sweeps of every variant and share count over 1 to 32 sequences, 1 to 128 new
+// tokens, windows of 512 tokens and contexts of 512 to 32768: a launch is about
+//   fixed + rounds * (start + page * pages of a share)
+// or, where that is longer, the bytes read once at 6.4 TB/s; a round is one workgroup on every compute unit, and where a second
+// one fits beside it (heads of 64) the two take (1 + beside) rounds.  More than one share adds the join.  The choice that this
+// predicts to be shortest was within 2 % of the best measured one on average and within 15 % in the worst of 82 calls; fixed
+// thresholds on rows and pages were 15 % off on average and lost up to 1.7 times (1 token, 8 KV heads of 128, 4096 tokens: 8
+// shares 12.9 us, 32 shares 8.5; 16 tokens, 2 KV heads of 64, window 512: 32 rows a workgroup 10.1, 16 rows 7.5).
+struct PagedCost {
+  int tiles, n;  // the tile kernel's wavefronts, or the row kernel's 16-row blocks
+  float fixed, start, page, beside;
+};
+static const PagedCost kPagedCost128[] = {{0, 1, 1.9f, 3.4f, 0.59f, 1.f}, {0, 2, 3.2f, 4.0f, 0.76f, 1.f}, {1, 2, 3.7f, 2.5f, 1.11f, 1.f},
+                                          {1, 4, 4.4f, 2.4f, 1.18f, 1.f}, {1, 8, 3.1f, 4.0f, 1.59f, 1.f}};
+static const PagedCost kPagedCost64[] = {{0, 1, 3.3f, 1.4f, 0.28f, 1.f}, {0, 2, 4.3f, 1.5f, 0.48f, 0.4f}, {1, 2, 3.7f, 2.4f, 0.85f, 0.4f},
+                                         {1, 4, 4.9f, 1.8f, 0.88f, 0.5f}};
+
+static PagedPlan paged_plan(int B, int T, int HQ, int H, int D, int window, int max_pages) {
+  PagedPlan best = {};
+  const int G = HQ / H;
+  const long rows = (long)T * G, cus = hils_device_cus();
+  const auto pages_of = [&](long tokens) {  // pages that `tokens` new tokens and the window before them can lie on
+    const long pages = ((long)window + tokens + 2 * PA_PAGE - 3) / PA_PAGE;
+    return pages < max_pages ? pages : max_pages;
+  };
+  const float read = (float)B * H * pages_of(T) * PA_PAGE * D * 4 / 6.4e6f;
+  float least = 0.f;
+  const PagedCost* cost = D == 128 ? kPagedCost128 : kPagedCost64;
+  for (int i = 0; i < (D == 128 ? 5 : 4); ++i) {
+    const PagedCost& c = cost[i];
+    const int per = c.tiles ? 32 * c.n : 16 * c.n;
+    if (i && rows <= per / 2) break;  // (the variants before hold every row with fewer of them empty)
+    const long n_blk = (rows + per - 1) / per, tokens = per / G + 1 > PA_MAX_TREE ? per / G + 1 : PA_MAX_TREE;
+    const long pages = pages_of(T < tokens ? T : tokens);
+    for (int n_split = 1; n_split <= 64 && (n_split == 1 || 2 * n_split <= pages); n_split += n_split < 4 ? 1 : n_split / 4) {
+      const long n = (n_blk * n_split * H * B + cus - 1) / cus;
+      const float rounds = c.beside < 1.f ? (n / 2) * (1.f + c.beside) + n % 2 : (float)n;
+      const float work = rounds * (c.start + c.page * ((pages + n_split - 1) / n_split));
+      // (the fourth powers: a sweep near both bounds takes longer than either)
+      float t = c.fixed + sqrtf(sqrtf(work * work * work * work + read * read * read * read));
+      if (n_split > 1) t += 2.4f + (float)B * rows * H * n_split * (D + 2) * 8 / 3.7e6f;
+      if (best.n_blk && t >= least) continue;
+      least = t;
+      best.tiles = c.tiles;
+      best.nr = best.nw = c.n;
+      best.n_blk = (int)n_blk;
+      best.n_split = n_split;
+    }
+  }
+  return best;
 }
 
 static size_t paged_ws(const PagedPlan& pl, long rows, int D) {
@@ -813,26 +972,33 @@ static size_t paged_ws(const PagedPlan& pl, long rows, int D) {
 
 extern "C" size_t hils_paged_attn_workspace(int B, int T, int HQ, int H, int D, int window, int max_pages) {
   if (B <= 0 || T <= 0 || H <= 0 || HQ <= 0 || HQ % H != 0 || window <= 0 || max_pages <= 0) return 0;
-  return paged_ws(paged_plan(B, T, HQ, H, window, max_pages), (long)B * T * HQ, D);
+  return paged_ws(paged_plan(B, T, HQ, H, D, window, max_pages), (long)B * T * HQ, D);
 }
 
 template <int D, bool TREE>
 static int paged_launch(const PagedPlan& pl, const bf16_t* q, const bf16_t* k, const bf16_t* v, const PagedDims& dm,
                         const PagedOut& out, hipStream_t st) {
+  const dim3 grid((unsigned)(((long)dm.n_blk * dm.n_split * dm.H * dm.B + 7) / 8 * 8));
   if (pl.tiles) {
-    auto kern = paged_attn_tiles<D, TREE>;
-    static HilsLdsReserve reserved;
-    if (int rc = hils_reserve_lds(&reserved, (const void*)kern, paged_tiles_smem<D>(), "hils_paged_attn")) return rc;
-    const long total = (long)dm.n_blk * dm.n_split * dm.H * dm.B;
-    hipLaunchKernelGGL(kern, dim3((unsigned)((total + 7) / 8 * 8)), dim3(256), paged_tiles_smem<D>(), st, q, k, v, dm, out);
+#define PA_TILES(NW_)                                                                                                     \
+  do {                                                                                                                   \
+    static HilsLdsReserve reserved;                                                                                      \
+    constexpr size_t smem = paged_tiles_smem<D, NW_, TREE>();                                                            \
+    if (int rc = hils_reserve_lds(&reserved, (const void*)paged_attn_tiles<D, NW_, TREE>, smem, "hils_paged_attn")) return rc; \
+    hipLaunchKernelGGL((paged_attn_tiles<D, NW_, TREE>), grid, dim3(NW_ * 64), smem, st, q, k, v, dm, out);              \
+  } while (0)
+    if constexpr (D == 128) {
+      if (pl.nw == 8) PA_TILES(8);
+    }
+    if (pl.nw == 4) PA_TILES(4);
+    if (pl.nw == 2) PA_TILES(2);
+#undef PA_TILES
   } else {
-    const dim3 grid(dm.n_blk * dm.n_split, dm.H, dm.B);
     if (pl.nr == 1) hipLaunchKernelGGL((paged_attn_rows<D, 1, 8, TREE>), grid, dim3(512), 0, st, q, k, v, dm, out);
     else hipLaunchKernelGGL((paged_attn_rows<D, 2, 4, TREE>), grid, dim3(256), 0, st, q, k, v, dm, out);
   }
   if (dm.n_split > 1) {
-    const int per = 256 / (D / 4);
-    hipLaunchKernelGGL((paged_attn_join<D>), dim3((unsigned)((out.n_rows + per - 1) / per)), dim3(256), 0, st, out, dm.n_split, dm.c2);
+    hipLaunchKernelGGL((paged_attn_join<D>), dim3((unsigned)((out.n_rows + 3) / 4)), dim3(256), 0, st, out, dm.n_split, dm.c2);
   }
   return HILS_OK;
 }
@@ -856,7 +1022,7 @@ extern "C" int hils_paged_attn(const void* q, const void* k_pages, const void* v
   HILS_REQUIRE(B <= 65535 && H <= 65535 && (long)T * (HQ / H) * (HQ / H) < (1l << 31), "hils_paged_attn: sizes too large for the grid");
   HILS_REQUIRE(q_batch_stride % 8 == 0 && q_token_stride % 8 == 0 && q_head_stride % 8 == 0 && (uintptr_t)q % 16 == 0,
                "hils_paged_attn: q's strides and address must be multiples of 16 bytes");
-  const PagedPlan pl = paged_plan(B, T, HQ, H, window, max_pages);
+  const PagedPlan pl = paged_plan(B, T, HQ, H, D, window, max_pages);
   const long rows = (long)B * T * HQ;
   HILS_REQUIRE((long)pl.n_blk * pl.n_split * H * B < (1l << 31) - 8, "hils_paged_attn: sizes too large for the grid");
   const size_t need = paged_ws(pl, rows, D);

@@ -27,10 +27,8 @@ struct RotaryDims {
   const int32_t* lengths;                     // (B) or null: seq_len
 };
 
-#ifndef ROT_UN
 #define ROT_UN 2
 #define ROT_WAVES 4
-#endif
 
 // Eight pairs of a unit.  The rounding fp64 -> fp32 -> bf16 differs from the one to bf16 only where the first lands halfway
 // between two bf16 values: true if some value did (about one in 65536), and with FIX such a value goes the way it came from.
