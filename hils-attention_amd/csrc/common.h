@@ -42,6 +42,9 @@ struct HilsLdsReserve { std::atomic<size_t> bytes[HILS_LDS_RESERVE_DEVICES]; };
 int hils_reserve_lds(HilsLdsReserve* state, const void* kernel, size_t bytes, const char* who);
 #endif
 
+// Bytes that the last-level cache in front of the HBM holds.  What is read or written once and is larger does better past it.
+#define HILS_LAST_CACHE (256l << 20)
+
 typedef unsigned short bf16_t;  // raw bfloat16 bits
 
 #define HILS_NEG_INF (-INFINITY)

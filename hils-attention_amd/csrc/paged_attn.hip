@@ -18,6 +18,8 @@
 // Values at slots that a row does not see meet a probability of exactly 0, which an infinity or a NaN there (a stale slot
 // behind the last token, a rejected draft) would turn into a NaN.  A row whose result is no finite number is therefore
 // computed once more, token by token over the slots that it sees alone (paged_redo_row): the common call pays a comparison.
+#include <string.h>
+
 #include "common.h"
 #include "lds_dma.h"
 #include "../../include/hils_amd.h"
@@ -248,7 +250,7 @@ __device__ __forceinline__ void paged_redo_row(const PagedDims& dm, const PagedO
 // 16 NR rows a workgroup; units of 32 tokens (half a page) go to its wavefronts in turn, the next unit's keys and values
 // under way while one is worked on; the wavefronts' results meet in LDS.  K rows are read straight into A operands (a lane 16
 // bytes of its token's row), V goes through the wavefront's own LDS area and is read by the transposing load.
-template <int D, int NR, int NWV, bool TREE>
+template <int D, int NR, int NWV, bool TREE, bool PAST>
 __global__ void __launch_bounds__(NWV * 64) __attribute__((amdgpu_waves_per_eu(NR == 2 && D == 128 ? 1 : 2)))
 paged_attn_rows(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, const bf16_t* __restrict__ v, PagedDims dm,
                 PagedOut out) {
@@ -306,7 +308,7 @@ paged_attn_rows(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, cons
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) kd[tt][ks] = *(const pa_u4*)(kp + tt * 16 * D + ks * 32);
 #pragma unroll
-    for (int i = 0; i < VI; ++i) vd[i] = *(const pa_u4*)(vp + i * TPI * D);
+    for (int i = 0; i < VI; ++i) vd[i] = PAST ? __builtin_nontemporal_load((const pa_u4*)(vp + i * TPI * D)) : *(const pa_u4*)(vp + i * TPI * D);
   };
 
   unsigned char* area = area_s + wave * AREA;
@@ -909,7 +911,7 @@ __global__ void __launch_bounds__(256) paged_attn_join(PagedOut out, int n_split
 
 // ---- host ----------------------------------------------------------------------------------------
 struct PagedPlan {
-  bool tiles;
+  bool tiles, past;            // past: values are read past the caches
   int nr, nw, n_blk, n_split;  // 16 nr rows a workgroup, or 32 nw
 };
 
@@ -931,7 +933,7 @@ static const PagedCost kPagedCost128[] = {{0, 1, 1.9f, 3.4f, 0.59f, 1.f}, {0, 2,
 static const PagedCost kPagedCost64[] = {{0, 1, 3.3f, 1.4f, 0.28f, 1.f}, {0, 2, 4.3f, 1.5f, 0.48f, 0.4f}, {1, 2, 3.7f, 2.4f, 0.85f, 0.4f},
                                          {1, 4, 4.9f, 1.8f, 0.88f, 0.5f}};
 
-static PagedPlan paged_plan(int B, int T, int HQ, int H, int D, int window, int max_pages) {
+static PagedPlan paged_choose(int B, int T, int HQ, int H, int D, int window, int max_pages) {
   PagedPlan best = {};
   const int G = HQ / H;
   const long rows = (long)T * G, cus = hils_device_cus();
@@ -963,7 +965,24 @@ static PagedPlan paged_plan(int B, int T, int HQ, int H, int D, int window, int 
       best.n_split = n_split;
     }
   }
+  // One row block reads a key and a value once.  Where all of them do not fit the last cache, values go past it: 16 sequences of
+  // 16K to 32K, 8 KV heads of 128 (1.54 GB): 277 -> 255 us; where they fit, and are there from the call before, that would lose
+  // (32768 tokens, 8 heads of 128: 28 -> 33 us).  Keys are read 64 bytes of a row at a time, half a cache line, and lose by it
+  // at any size.
+  best.past = best.n_blk == 1 && (double)B * H * pages_of(T) * PA_PAGE * D * 4 > HILS_LAST_CACHE;
   return best;
+}
+
+// (The choice takes 0.6 us; a thread that asks for the same sizes again, as a workspace's size and the call do, gets the same.)
+static PagedPlan paged_plan(int B, int T, int HQ, int H, int D, int window, int max_pages) {
+  static thread_local int sizes[8];
+  static thread_local PagedPlan plan;
+  const int now[8] = {B, T, HQ, H, D, window, max_pages, hils_device_cus()};
+  if (memcmp(sizes, now, sizeof(now))) {
+    plan = paged_choose(B, T, HQ, H, D, window, max_pages);
+    memcpy(sizes, now, sizeof(now));
+  }
+  return plan;
 }
 
 static size_t paged_ws(const PagedPlan& pl, long rows, int D) {
@@ -994,8 +1013,9 @@ static int paged_launch(const PagedPlan& pl, const bf16_t* q, const bf16_t* k, c
     if (pl.nw == 2) PA_TILES(2);
 #undef PA_TILES
   } else {
-    if (pl.nr == 1) hipLaunchKernelGGL((paged_attn_rows<D, 1, 8, TREE>), grid, dim3(512), 0, st, q, k, v, dm, out);
-    else hipLaunchKernelGGL((paged_attn_rows<D, 2, 4, TREE>), grid, dim3(256), 0, st, q, k, v, dm, out);
+    if (pl.nr == 1 && pl.past) hipLaunchKernelGGL((paged_attn_rows<D, 1, 8, TREE, true>), grid, dim3(512), 0, st, q, k, v, dm, out);
+    else if (pl.nr == 1) hipLaunchKernelGGL((paged_attn_rows<D, 1, 8, TREE, false>), grid, dim3(512), 0, st, q, k, v, dm, out);
+    else hipLaunchKernelGGL((paged_attn_rows<D, 2, 4, TREE, false>), grid, dim3(256), 0, st, q, k, v, dm, out);
   }
   if (dm.n_split > 1) {
     hipLaunchKernelGGL((paged_attn_join<D>), dim3((unsigned)((out.n_rows + 3) / 4)), dim3(256), 0, st, out, dm.n_split, dm.c2);

@@ -5,7 +5,9 @@
 // ---- whole pages -------------------------------------------------------------------------------
 // pool[dst[i]] = pool[src[i]] for every i and up to eight pools at once.  Bound by HBM (every byte read and written once)
 // or, for a few pages, by the one launch.  A workgroup copies one piece of 32 KiB of a pair of pages, its eight 16-byte
-// loads per thread in flight together.
+// loads per thread in flight together.  Moves larger than the last cache go past it: 2048 pages of 2 x 128 KiB and small
+// pools (1.08 GB read and written) in 208 us (5.2 TB/s), 217 through the caches; a fork of 32 pages takes 5 us either way and
+// its pages are read next.
 typedef unsigned pg_u4 __attribute__((ext_vector_type(4)));
 #define PC_POOLS 8
 #define PC_PIECE 32768
@@ -16,12 +18,13 @@ struct PageCopy {
   int first[PC_POOLS + 1];    // first piece of a pool among the pieces of a pair
   int unit[PC_POOLS];         // 16, 4 or 1: what every page of the pool is a whole number of, and aligned to
   int n_pools, num_pages, wide;
+  int past;                   // past the caches: what is read and written does not fit the last of them
   uint32_t m_pieces;
   const void* src;
   const void* dst;
 };
 
-template <typename V>
+template <typename V, bool PAST>
 __device__ __forceinline__ void page_copy_piece(unsigned char* to, const unsigned char* from, int bytes) {
   const V* f = (const V*)from;
   V* t = (V*)to;
@@ -30,10 +33,13 @@ __device__ __forceinline__ void page_copy_piece(unsigned char* to, const unsigne
     V x[8];
 #pragma unroll
     for (int u = 0; u < 8; ++u)
-      if (i0 + 256 * u < n) x[u] = f[i0 + 256 * u];
+      if (i0 + 256 * u < n) x[u] = PAST ? __builtin_nontemporal_load(f + i0 + 256 * u) : f[i0 + 256 * u];
 #pragma unroll
     for (int u = 0; u < 8; ++u)
-      if (i0 + 256 * u < n) t[i0 + 256 * u] = x[u];
+      if (i0 + 256 * u < n) {
+        if (PAST) __builtin_nontemporal_store(x[u], t + i0 + 256 * u);
+        else t[i0 + 256 * u] = x[u];
+      }
   }
 }
 
@@ -49,9 +55,10 @@ __global__ void __launch_bounds__(256) page_copy_kernel(PageCopy pc) {
   const int bytes = left < PC_PIECE ? (int)left : PC_PIECE;
   const unsigned char* from = pc.pool[p] + src * pc.bytes[p] + at;
   unsigned char* to = pc.pool[p] + dst * pc.bytes[p] + at;
-  if (pc.unit[p] == 16) page_copy_piece<pg_u4>(to, from, bytes);
-  else if (pc.unit[p] == 4) page_copy_piece<uint32_t>(to, from, bytes);
-  else page_copy_piece<unsigned char>(to, from, bytes);
+  if (pc.unit[p] == 16 && pc.past) page_copy_piece<pg_u4, true>(to, from, bytes);
+  else if (pc.unit[p] == 16) page_copy_piece<pg_u4, false>(to, from, bytes);
+  else if (pc.unit[p] == 4) page_copy_piece<uint32_t, false>(to, from, bytes);
+  else page_copy_piece<unsigned char, false>(to, from, bytes);
 }
 
 extern "C" int hils_copy_pages(void** pools, const size_t* page_bytes, const void* src, const void* dst, int n_pools, int n,
@@ -71,6 +78,9 @@ extern "C" int hils_copy_pages(void** pools, const size_t* page_bytes, const voi
     HILS_REQUIRE(pc.first[i] + pieces < (1 << 26), "hils_copy_pages: pages too large");
     pc.first[i + 1] = pc.first[i] + (int)pieces;
   }
+  double moved = 0;
+  for (int i = 0; i < n_pools; ++i) moved += 2. * pc.bytes[i] * n;
+  pc.past = moved > HILS_LAST_CACHE;
   const long blocks = (long)pc.first[n_pools] * n;
   HILS_REQUIRE(blocks <= 2147483647L && blocks * pc.first[n_pools] < (1l << 32), "hils_copy_pages: too much for one call");
   pc.n_pools = n_pools;

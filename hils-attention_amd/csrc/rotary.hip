@@ -7,8 +7,8 @@
 //
 // The angle of a far position has lost its fraction of a turn in fp32 (position 10^6, inv_freq 1: steps of 0.06), so it is
 // formed in turns in fp64 and reduced to [-1/2, 1/2] there; the rotation is fp64 too (fp32's rate on this chip, and the kernel
-// waits for memory), so that what is rounded to bf16, once, is the exact value: a key in the cache is the same whatever
-// computed it.
+// waits for memory), so that what is rounded to bf16 is the exact value: a key in the cache is the same whatever computed
+// it.
 // Bound by HBM: q and k in and out.  A workgroup owns a few tokens of all heads; their R/2 angles each are worked out
 // once, into LDS, for all heads (an angle costs some 60 instructions: per head they would be most of the kernel).  A
 // thread's unit is 16 features that go together: two 16-byte pieces in and out, four units' loads in flight.
@@ -30,36 +30,20 @@ struct RotaryDims {
 #define ROT_UN 2
 #define ROT_WAVES 4
 
-// Eight pairs of a unit.  The rounding fp64 -> fp32 -> bf16 differs from the one to bf16 only where the first lands halfway
-// between two bf16 values: true if some value did (about one in 65536), and with FIX such a value goes the way it came from.
-template <bool INTERLEAVED, bool FIX>
-__device__ __forceinline__ bool rotary_turn(const uint4 lo, const uint4 hi, const double* c, const double* s, uint4& out_lo,
+// Eight pairs of a unit.  What is exact to 2^-53 goes to bf16 by way of fp32, as a conversion from fp64 does: half a step of
+// bf16 and at most 2^-24 more.
+template <bool INTERLEAVED>
+__device__ __forceinline__ void rotary_turn(const uint4 lo, const uint4 hi, const double* c, const double* s, uint4& out_lo,
                                             uint4& out_hi) {
   float a[8], b[8], y1[8], y2[8];
   unpack8(lo, a);
   unpack8(hi, b);
-  bool tie = false;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const double x1 = INTERLEAVED ? (i < 4 ? a[2 * i & 7] : b[2 * i & 7]) : a[i];
     const double x2 = INTERLEAVED ? (i < 4 ? a[(2 * i + 1) & 7] : b[(2 * i + 1) & 7]) : b[i];
-    const double d1 = fma(x1, c[i], -(x2 * s[i])), d2 = fma(x2, c[i], x1 * s[i]);
-    float f1 = (float)d1, f2 = (float)d2;
-    if (FIX) {
-      auto fix = [](double d, float f) {
-        unsigned u = __float_as_uint(f);
-        const double back = f;
-        if ((u & 0xffffu) == 0x8000u && d != back) u += (d > back) == (f > 0.f) ? 1u : -1u;
-        return __uint_as_float(u);
-      };
-      f1 = fix(d1, f1);
-      f2 = fix(d2, f2);
-    } else {
-      tie |= (__float_as_uint(f1) & 0xffffu) == 0x8000u;
-      tie |= (__float_as_uint(f2) & 0xffffu) == 0x8000u;
-    }
-    y1[i] = f1;
-    y2[i] = f2;
+    y1[i] = (float)fma(x1, c[i], -(x2 * s[i]));
+    y2[i] = (float)fma(x2, c[i], x1 * s[i]);
   }
   unsigned* wl = (unsigned*)&out_lo;
   unsigned* wh = (unsigned*)&out_hi;
@@ -68,7 +52,6 @@ __device__ __forceinline__ bool rotary_turn(const uint4 lo, const uint4 hi, cons
     wl[i] = INTERLEAVED ? pack_bf2(y1[i], y2[i]) : pack_bf2(y1[2 * i], y1[2 * i + 1]);
     wh[i] = INTERLEAVED ? pack_bf2(y1[4 + i], y2[4 + i]) : pack_bf2(y2[2 * i], y2[2 * i + 1]);
   }
-  return tie;
 }
 
 template <bool INTERLEAVED, bool APPEND>
@@ -173,8 +156,7 @@ rotary_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, const 
         const double* c = cos_s + tab[x];
         const double* sn = sin_s + tab[x];
         const uint4 l0 = lo[x], h0 = hi[x];
-        if (rotary_turn<INTERLEAVED, false>(l0, h0, c, sn, lo[x], hi[x]))
-          rotary_turn<INTERLEAVED, true>(l0, h0, c, sn, lo[x], hi[x]);
+        rotary_turn<INTERLEAVED>(l0, h0, c, sn, lo[x], hi[x]);
       }
       if (late[x] >= 0) {
         const long at = slot_s[late[x]];

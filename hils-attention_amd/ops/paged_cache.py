@@ -23,9 +23,7 @@ class _NoBackward(torch.autograd.Function):
 
 
 def _inference(name, call, *inputs):
-    if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in inputs):
-        return _NoBackward.apply(name, call, *inputs)
-    return call()
+    return _NoBackward.apply(name, call, *inputs) if torch.is_grad_enabled() else call()
 
 
 def paged_append(k, v, k_pages, v_pages, page_table, seq_len, q=None, inv_freq=None, positions=None, interleaved=False,
@@ -33,8 +31,10 @@ def paged_append(k, v, k_pages, v_pages, page_table, seq_len, q=None, inv_freq=N
     """Write keys and values (B,T,H,D) of the last T of ``seq_len`` tokens into their pages, in one launch; tokens whose
     page is not mapped are left out.  With ``inv_freq`` the keys, and q (B,T,H_q,D) if given, are rotated on the way as by
     ``rotary_embedding``, at ``positions`` (B,T) or, without them, at the tokens' slots.  Returns the rotated q or None."""
-    return _inference("paged_append", lambda: _cabi.host().paged_append(
-        k, v, k_pages, v_pages, page_table, seq_len, q, inv_freq, positions, bool(interleaved), float(scale)), q, k, v)
+    args = (k, v, k_pages, v_pages, page_table, seq_len, q, inv_freq, positions, bool(interleaved), float(scale))
+    if k.requires_grad or v.requires_grad or (q is not None and q.requires_grad):
+        return _inference("paged_append", lambda: _cabi.host().paged_append(*args), q, k, v)
+    return _cabi.host().paged_append(*args)
 
 
 def paged_flex_attn(q, k_pages, v_pages, page_table, seq_len, window_size, parents=None, mask_lmk=True,
@@ -47,8 +47,10 @@ def paged_flex_attn(q, k_pages, v_pages, page_table, seq_len, window_size, paren
     seq_len - T + depth and sees the committed tokens of its window, itself and its ancestors.  Tokens with any other parent,
     and those that follow them, see nothing (padding).  Without ``parents`` the tokens are a chain.  T <= 256 for a tree.
     Returns o (B,T,H_q,D) bf16 and lse (B,T,H_q) fp32, natural log; rows that see nothing: 0 and -inf."""
-    return _inference("paged_flex_attn", lambda: _cabi.host().paged_flex_attn(
-        q, k_pages, v_pages, page_table, seq_len, int(window_size), parents, bool(mask_lmk), bool(expand_to_chunk), sm_scale), q)
+    args = (q, k_pages, v_pages, page_table, seq_len, int(window_size), parents, bool(mask_lmk), bool(expand_to_chunk), sm_scale)
+    if q.requires_grad:
+        return _inference("paged_flex_attn", lambda: _cabi.host().paged_flex_attn(*args), q)
+    return _cabi.host().paged_flex_attn(*args)
 
 
 def paged_accept(k_pages, v_pages, page_table, base_len, path):

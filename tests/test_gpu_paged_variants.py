@@ -14,7 +14,7 @@ CASES = [(32, 8, 2, 64, 512, 1024), (32, 8, 8, 33, 1 << 20, 900), (32, 8, 8, 64,
          (4, 4, 5, 200, 1 << 20, 900), (6, 2, 5, 100, 1 << 20, 4500), (32, 8, 3, 33, 1 << 20, 4500), (5, 1, 16, 33, 1 << 20, 4500),
          (32, 8, 1, 33, 1 << 20, 18000), (32, 8, 2, 33, 1 << 20, 9000), (4, 4, 1, 33, 1 << 20, 18000), (6, 2, 2, 33, 1 << 20, 18000),
          (5, 1, 2, 33, 1 << 20, 18000), (4, 4, 16, 33, 1 << 20, 18000), (32, 8, 16, 7, 1 << 20, 4500), (32, 8, 8, 7, 1 << 20, 18000),
-         (4, 4, 16, 1, 1 << 20, 18000), (5, 1, 1, 1, 1 << 20, 18000), (32, 8, 16, 40, 1 << 20, 9000)]
+         (4, 4, 16, 1, 1 << 20, 18000), (5, 1, 1, 1, 1 << 20, 18000), (32, 8, 16, 40, 1 << 20, 9000), (32, 8, 16, 4, 1 << 20, 9000)]
 
 
 def _inputs(dev, D, HQ, H, B, T, ctx, tree, seed):

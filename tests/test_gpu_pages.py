@@ -35,6 +35,22 @@ def test_copy_pages(pkg, dev, n, wide):
     assert torch.equal(pools[0][2:4], want[0][:2])
 
 
+def test_more_than_the_last_cache_holds(pkg, dev):
+    note("a move of 330 MB, read and written")
+    gen = torch.Generator(device=dev).manual_seed(3)
+    P, n = 2603, 1300
+    pools = [torch.randint(0, 256, (P, 127008), device=dev, dtype=torch.uint8, generator=gen),
+             torch.randn(P, 33, device=dev, generator=gen)]
+    order = torch.randperm(P, device=dev, generator=gen)
+    src, dst = order[:n], order[n:2 * n]
+    want = [p.clone() for p in pools]
+    for p in want:
+        p[dst] = p[src]
+    for _ in range(2):  # (nothing that is written is read: once more changes nothing)
+        pkg.copy_pages(pools, src, dst)
+        assert all(torch.equal(a, b) for a, b in zip(pools, want))
+
+
 def test_copy_views(pkg, dev):
     note("a pool that begins between two multiples of 16 bytes")
     whole = torch.randn(1 + 10 * 33, device=dev).bfloat16()
