@@ -32,7 +32,7 @@ typedef short pa_s4 __attribute__((ext_vector_type(4)));
 typedef short pa_s8 __attribute__((ext_vector_type(8)));
 
 struct PagedDims {
-  int B, T, HQ, H, G, window, expand, mask_lmk, max_pages, num_pages, seq_len, n_blk, n_split, parents_stride;
+  int B, T, HQ, H, G, window, expand, mask_lmk, max_pages, num_pages, seq_len, n_blk, n_split, ragged, parents_stride;
   uint32_t g_magic;
   float c2;                     // scale * log2(e)
   long q_sb, q_st, q_sh;        // elements between sequences, tokens and heads of q
@@ -47,44 +47,95 @@ struct PagedSpan {
   bool alive;
 };
 
-// What a workgroup works on.  The row blocks of a (sequence, KV head, share) read the same pages: neighbours on one XCD (the
-// hardware hands consecutive workgroups to the eight XCDs in turn).  False for the padding at the end.
-struct PagedUnit {
-  int blk, share, hk, b;
-};
-__device__ __forceinline__ bool paged_unit(const PagedDims& dm, PagedUnit& u) {
-  const int total = dm.n_blk * dm.n_split * dm.H * dm.B, per_xcd = (total + 7) / 8;
-  const int id = (int)(blockIdx.x % 8) * per_xcd + (int)(blockIdx.x / 8);
-  if (id >= total) return false;
-  const int rest = id / dm.n_blk, pair = rest / dm.n_split;
-  u.blk = id - rest * dm.n_blk;
-  u.share = rest - pair * dm.n_split;
-  u.b = pair / dm.H;
-  u.hk = pair - u.b * dm.H;
-  return true;
-}
-
 __device__ __forceinline__ int paged_left(int p, const PagedDims& dm) {
   const int left = p - dm.window + 1;
   return dm.expand ? left & -PA_PAGE : left;
 }
 
-__device__ __forceinline__ PagedSpan paged_span(const PagedDims& dm, int b, int r0, int r1, int share) {
+// Slots [lo, hi) that the tokens t0 .. t1 of a sequence of `len` see, and their pages from lo / PA_PAGE on.
+__device__ __forceinline__ int paged_pages(const PagedDims& dm, int len, int t0, int t1, int& lo, int& hi) {
+  const int base = len - dm.T, left = paged_left(base + t0, dm);
+  lo = left > 0 ? left : 0;
+  const long end = (long)dm.max_pages * PA_PAGE;
+  hi = base + t1 + 1 < end ? base + t1 + 1 : (int)end;
+  const int n = len >= dm.T ? (hi + PA_PAGE - 1) / PA_PAGE - lo / PA_PAGE : 0;
+  return n > 0 ? n : 0;
+}
+
+// Sums over the lanes up to this one.
+__device__ __forceinline__ int paged_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);  // from 1, 2, 4, 8 lanes before, in rows of 16
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // a row's last sum to the row behind it,
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // that of two rows to the two behind them
+  return x;
+}
+
+// Shares of a ragged batch, up to 64 sequences, lane b's of sequence b: n_split a sequence on average, as many as make the
+// longest share shortest.  With c pages a share a sequence of n pages needs ceil(n / c); c lies between all / (n_split B) and
+// all / ((n_split - 1) B), where sum (1 + (n - 1) / c) < B + (n_split - 1) B fits in any case; five halvings come within 4 % of
+// the best c.  Equal numbers of shares leave the longest sequence's workgroups alone at the end: trees of 64 tokens for four
+// sequences of 8K to 16K (8 shares on average), see the tile kernel's figures.
+__device__ __forceinline__ int paged_ragged(const PagedDims& dm, int lane, int len) {
+  int lo, hi;
+  const int n = lane < dm.B ? paged_pages(dm, len, 0, dm.T - 1, lo, hi) : 0;
+  const int slots = dm.n_split * dm.B;
+  const int sum = __builtin_amdgcn_readlane(paged_scan(n), 63);
+  const float all = (float)(sum > 1 ? sum : 1), rest = n > 1 ? (float)(n - 1) : 0.f;
+  const auto shares = [&](float c) __attribute__((always_inline)) {
+    return lane < dm.B ? 1 + (int)fminf(rest * __builtin_amdgcn_rcpf(c), 63.f) : 0;
+  };
+  float few = all / (float)slots, fit = all / (float)(slots - dm.B) * (1.f + 0x1p-18f);
+  for (int i = 0; i < 5; ++i) {
+    const float c = 0.5f * (few + fit);
+    if (__builtin_amdgcn_readlane(paged_scan(shares(c)), 63) <= slots) fit = c;
+    else few = c;
+  }
+  return shares(fit);
+}
+
+// What a workgroup works on: share `share` of `of` of a sequence's pages.  The row blocks of a (share, KV head) read the same
+// pages: neighbours on one XCD (the hardware hands consecutive workgroups to the eight XCDs in turn).  `slot` numbers the
+// shares of all sequences (it is the sequence where none is split).  False for what is left over at the end.
+struct PagedUnit {
+  int blk, hk, slot, b, share, of, len;
+};
+__device__ __forceinline__ bool paged_unit(const PagedDims& dm, int lane, PagedUnit& u) {
+  const int total = dm.n_blk * dm.n_split * dm.H * dm.B, per_xcd = (total + 7) / 8;
+  const int id = (int)(blockIdx.x % 8) * per_xcd + (int)(blockIdx.x / 8);
+  if (id >= total) return false;
+  const int rest = id / dm.n_blk;
+  u.blk = id - rest * dm.n_blk;
+  u.slot = rest / dm.H;
+  u.hk = rest - u.slot * dm.H;
+  if (dm.ragged) {
+    const int len = lane < dm.B ? dm.lengths[lane] : 0;
+    const int n = paged_ragged(dm, lane, len), behind = paged_scan(n);
+    if (u.slot >= __builtin_amdgcn_readlane(behind, 63)) return false;
+    u.b = 63 - __builtin_clzll(__ballot(lane < dm.B && behind - n <= u.slot));
+    u.of = __builtin_amdgcn_readlane(n, u.b);
+    u.share = u.slot - __builtin_amdgcn_readlane(behind, u.b) + u.of;
+    u.len = __builtin_amdgcn_readlane(len, u.b);
+    return true;
+  }
+  u.b = u.slot / dm.n_split;
+  u.of = dm.n_split;
+  u.share = u.slot - u.b * dm.n_split;
+  u.len = dm.lengths ? dm.lengths[u.b] : dm.seq_len;
+  return true;
+}
+
+__device__ __forceinline__ PagedSpan paged_span(const PagedDims& dm, const PagedUnit& u, int r0, int r1) {
   PagedSpan sp;
-  const int len = dm.lengths ? dm.lengths[b] : dm.seq_len;
-  sp.base = len - dm.T;
-  sp.alive = len >= dm.T;
+  sp.base = u.len - dm.T;
+  sp.alive = u.len >= dm.T;
   const int t0 = dm.parents ? 0 : (int)hils_udiv(r0, dm.G, dm.g_magic);
   const int t1 = dm.parents ? dm.T - 1 : (int)hils_udiv(r1 - 1, dm.G, dm.g_magic);
-  int lo = paged_left(sp.base + t0, dm);
-  sp.lo = lo > 0 ? lo : 0;
-  const long end = (long)dm.max_pages * PA_PAGE;
-  sp.hi = sp.base + t1 + 1 < end ? sp.base + t1 + 1 : (int)end;
-  const int first = sp.lo / PA_PAGE;
-  int n = sp.alive ? (sp.hi + PA_PAGE - 1) / PA_PAGE - first : 0;
-  n = n > 0 ? n : 0;
-  const int per = (n + dm.n_split - 1) / dm.n_split;
-  const int a = share * per < n ? share * per : n;
+  const int n = paged_pages(dm, u.len, t0, t1, sp.lo, sp.hi), first = sp.lo / PA_PAGE;
+  const int per = (n + u.of - 1) / u.of;
+  const int a = u.share * per < n ? u.share * per : n;
   sp.p0 = first + a;
   sp.p1 = first + (a + per < n ? a + per : n);
   return sp;
@@ -155,18 +206,18 @@ __device__ __forceinline__ unsigned paged_bits(const unsigned* row, int off) {
 struct PagedOut {
   bf16_t* o;
   float* lse;
-  float* part;   // (rows, shares, D) fp32, then (rows, shares, 2): maximum (score units) and sum
+  float* part;   // (shares of all sequences, T, HQ, D) fp32, then (.., 2): maximum (score units) and sum
   long n_rows;
 };
 
 template <int D>
-__device__ __forceinline__ void paged_store4(const PagedDims& dm, const PagedOut& out, long row, int share, int d4, f32x4_t x,
-                                             float M, float L) {
+__device__ __forceinline__ void paged_store4(const PagedDims& dm, const PagedOut& out, long row, int d4, f32x4_t x, float M,
+                                             float L) {
   if (dm.n_split > 1) {
-    float* p = out.part + (row * dm.n_split + share) * D + d4 * 4;
+    float* p = out.part + row * D + d4 * 4;
     *(f32x4_t*)p = x;
     if (d4 == 0) {
-      float* ml = out.part + out.n_rows * dm.n_split * D + (row * dm.n_split + share) * 2;
+      float* ml = out.part + out.n_rows * dm.n_split * D + row * 2;
       ml[0] = M;
       ml[1] = L;
     }
@@ -184,7 +235,7 @@ __device__ __forceinline__ void paged_store4(const PagedDims& dm, const PagedOut
 template <int D>
 __device__ __forceinline__ void paged_redo_row(const PagedDims& dm, const PagedOut& out, const bf16_t* qr, const bf16_t* k,
                                             const bf16_t* v, const int32_t* table, int hk, int base, int p0, int p1, int t,
-                                            int left, const unsigned* mask_row, long row, int share, int lane) {
+                                            int left, const unsigned* mask_row, long row, int lane) {
   float m = HILS_NEG_INF, l = 0.f, x[D / 64];
 #pragma unroll
   for (int f = 0; f < D / 64; ++f) x[f] = 0.f;
@@ -230,11 +281,11 @@ __device__ __forceinline__ void paged_redo_row(const PagedDims& dm, const PagedO
     }
   }
   if (dm.n_split > 1) {
-    float* part = out.part + (row * dm.n_split + share) * D;
+    float* part = out.part + row * D;
 #pragma unroll
     for (int f = 0; f < D / 64; ++f) part[f * 64 + lane] = x[f];
     if (lane == 0) {
-      float* ml = out.part + out.n_rows * dm.n_split * D + (row * dm.n_split + share) * 2;
+      float* ml = out.part + out.n_rows * dm.n_split * D + row * 2;
       ml[0] = m;
       ml[1] = l;
     }
@@ -266,11 +317,11 @@ paged_attn_rows(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, cons
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, j = lane >> 4;
   PagedUnit at;
-  if (!paged_unit(dm, at)) return;
-  const int blk = at.blk, share = at.share, hk = at.hk, b = at.b;
+  if (!paged_unit(dm, lane, at)) return;
+  const int blk = at.blk, hk = at.hk, b = at.b;
   const int n_rows = dm.T * dm.G, r0 = blk * ROWS;
   const int r1 = r0 + ROWS < n_rows ? r0 + ROWS : n_rows;
-  const PagedSpan sp = paged_span(dm, b, r0, r1, share);
+  const PagedSpan sp = paged_span(dm, at, r0, r1);
   const int32_t* table = dm.table + (long)b * dm.max_pages;
   const int t0 = hils_udiv(r0, dm.G, dm.g_magic);
 
@@ -483,8 +534,8 @@ paged_attn_rows(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, cons
       for (int i = 0; i < 4; ++i) x[i] = fmaf(f, ow[i], x[i]);
     }
     const int t = hils_udiv(r, dm.G, dm.g_magic), g = r - t * dm.G;
-    const long row = ((long)b * dm.T + t) * dm.HQ + hk * dm.G + g;
-    paged_store4<D>(dm, out, row, share, d4, x, M, L);
+    const long row = ((long)at.slot * dm.T + t) * dm.HQ + hk * dm.G + g;
+    paged_store4<D>(dm, out, row, d4, x, M, L);
     const float all = (x[0] + x[1]) + (x[2] + x[3]);  // (no finite number if one of them is none)
     if (!(fabsf(all) < INFINITY)) atomicOr(&odd_s, 1u << rr);
   }
@@ -493,10 +544,10 @@ paged_attn_rows(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, cons
     for (int rr = wave; rr < r1 - r0; rr += NWV) {
       if (!(odd >> rr & 1)) continue;
       const int r = r0 + rr, t = hils_udiv(r, dm.G, dm.g_magic), g = r - t * dm.G;
-      const long row = ((long)b * dm.T + t) * dm.HQ + hk * dm.G + g;
+      const long row = ((long)at.slot * dm.T + t) * dm.HQ + hk * dm.G + g;
       int left = TREE ? left_s[t - t0] : paged_left(sp.base + t, dm);
       paged_redo_row<D>(dm, out, q + b * dm.q_sb + t * dm.q_st + (hk * dm.G + g) * dm.q_sh, k, v, table, hk, sp.base, sp.p0,
-                        sp.p1, t, left, TREE ? mask_s + (t - t0) * PA_WORDS : nullptr, row, share, lane);
+                        sp.p1, t, left, TREE ? mask_s + (t - t0) * PA_WORDS : nullptr, row, lane);
     }
   }
 }
@@ -531,11 +582,11 @@ paged_attn_tiles(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, con
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, h = lane >> 5;
   PagedUnit at;
-  if (!paged_unit(dm, at)) return;
-  const int blk = at.blk, share = at.share, hk = at.hk, b = at.b;
+  if (!paged_unit(dm, lane, at)) return;
+  const int blk = at.blk, hk = at.hk, b = at.b;
   const int n_rows = dm.T * dm.G, r0 = blk * ROWS;
   const int r1 = r0 + ROWS < n_rows ? r0 + ROWS : n_rows;
-  const PagedSpan sp = paged_span(dm, b, r0, r1, share);
+  const PagedSpan sp = paged_span(dm, at, r0, r1);
   const int32_t* table = dm.table + (long)b * dm.max_pages;
   const int t0 = hils_udiv(r0, dm.G, dm.g_magic);
 
@@ -828,7 +879,7 @@ paged_attn_tiles(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, con
   const hils_uint2v two = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_run), __float_as_uint(l_run), false, false);
   const float l = __uint_as_float(two.x) + __uint_as_float(two.y);
   const float m = ref / dm.c2;  // (score units, as the joined shares have it)
-  const long row = ((long)b * dm.T + my_t) * dm.HQ + hk * dm.G + my_g;
+  const long row = ((long)at.slot * dm.T + my_t) * dm.HQ + hk * dm.G + my_g;
   float all = 0.f;
 #pragma unroll
   for (int ft = 0; ft < FT; ++ft)
@@ -840,7 +891,7 @@ paged_attn_tiles(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, con
 #pragma unroll
       for (int i4 = 0; i4 < 4; ++i4) {
         const f32x4_t x = {acc[ft][4 * i4], acc[ft][4 * i4 + 1], acc[ft][4 * i4 + 2], acc[ft][4 * i4 + 3]};
-        paged_store4<D>(dm, out, row, share, ft * 8 + i4 * 2 + h, x, m, l);
+        paged_store4<D>(dm, out, row, ft * 8 + i4 * 2 + h, x, m, l);
       }
   }
   uint64_t odd = __ballot(r < r1 && !(fabsf(all) < INFINITY));
@@ -854,7 +905,7 @@ paged_attn_tiles(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, con
       const int left = TREE ? left_s[tr - t0] : paged_left(sp.base + tr, dm);
       paged_redo_row<D>(dm, out, q + b * dm.q_sb + tr * dm.q_st + (hk * dm.G + gr) * dm.q_sh, k, v, table, hk, sp.base, sp.p0,
                         sp.p1, tr, left, TREE ? mask_s + (tr - t0) * PA_WORDS : nullptr,
-                        ((long)b * dm.T + tr) * dm.HQ + hk * dm.G + gr, share, lane);
+                        ((long)at.slot * dm.T + tr) * dm.HQ + hk * dm.G + gr, lane);
     }
   }
 }
@@ -863,21 +914,28 @@ paged_attn_tiles(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, con
 // A wavefront a row: lane i weighs share i (there are up to 64), then groups of D / 4 lanes take every GR-th share, four loads
 // under way, and add up across the groups.
 template <int D>
-__global__ void __launch_bounds__(256) paged_attn_join(PagedOut out, int n_split, float c2) {
+__global__ void __launch_bounds__(256) paged_attn_join(PagedDims dm, PagedOut out) {
   constexpr int LPR = D / 4, GR = 64 / LPR;  // lanes per row of features, groups
-  const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int rows = dm.T * dm.HQ, at = blockIdx.x * 4 + (threadIdx.x >> 6), b = blockIdx.y;
   const int lane = threadIdx.x & 63, d4 = lane % LPR, gr = lane / LPR;
-  if (row >= out.n_rows) return;  // (a whole wavefront)
-  const float* ml = out.part + out.n_rows * n_split * D + row * n_split * 2;
-  const float* part = out.part + row * n_split * D + d4 * 4;
+  if (at >= rows) return;  // (a whole wavefront)
+  int n_split = dm.n_split, slot = b * n_split;
+  if (dm.ragged) {
+    const int n = paged_ragged(dm, lane, lane < dm.B ? dm.lengths[lane] : 0), behind = paged_scan(n);
+    n_split = __builtin_amdgcn_readlane(n, b);
+    slot = __builtin_amdgcn_readlane(behind, b) - n_split;
+  }
+  const long row = (long)b * rows + at, first = (long)slot * rows + at;
+  const float* ml = out.part + out.n_rows * dm.n_split * D + first * 2;
+  const float* part = out.part + first * D + d4 * 4;
   float m = HILS_NEG_INF, l = 0.f;
   if (lane < n_split) {
-    m = ml[2 * lane];
-    l = ml[2 * lane + 1];
+    m = ml[2l * lane * rows];
+    l = ml[2l * lane * rows + 1];
   }
   const float M = wave_max(m);
   // (a share that saw nothing counts for nothing, whatever lies there)
-  const float f = l == 0.f ? 0.f : M > HILS_NEG_INF ? __builtin_amdgcn_exp2f((m - M) * c2) : 1.f;
+  const float f = l == 0.f ? 0.f : M > HILS_NEG_INF ? __builtin_amdgcn_exp2f((m - M) * dm.c2) : 1.f;
   const float L = wave_sum(l == 0.f ? 0.f : f * l);
   f32x4_t x = {0.f, 0.f, 0.f, 0.f};
   for (int s0 = gr; s0 < n_split + gr; s0 += 4 * GR) {
@@ -888,7 +946,7 @@ __global__ void __launch_bounds__(256) paged_attn_join(PagedOut out, int n_split
       const int s = s0 + u * GR;
       w[u] = __shfl(f, s & 63, 64);
       w[u] = s < n_split ? w[u] : 0.f;
-      y[u] = *(const f32x4_t*)(part + (long)(s < n_split ? s : 0) * D);
+      y[u] = *(const f32x4_t*)(part + (long)(s < n_split ? s : 0) * rows * D);
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u)
@@ -906,7 +964,7 @@ __global__ void __launch_bounds__(256) paged_attn_join(PagedOut out, int n_split
   pk.x = pack_bf2(x[0] * inv, x[1] * inv);
   pk.y = pack_bf2(x[2] * inv, x[3] * inv);
   *(uint2*)(out.o + row * D + d4 * 4) = pk;
-  if (d4 == 0) out.lse[row] = L == 0.f ? HILS_NEG_INF : (M * c2 + __builtin_amdgcn_logf(L)) * HILS_LN2;
+  if (d4 == 0) out.lse[row] = L == 0.f ? HILS_NEG_INF : (M * dm.c2 + __builtin_amdgcn_logf(L)) * HILS_LN2;
 }
 
 // ---- host ----------------------------------------------------------------------------------------
@@ -1018,7 +1076,7 @@ static int paged_launch(const PagedPlan& pl, const bf16_t* q, const bf16_t* k, c
     else hipLaunchKernelGGL((paged_attn_rows<D, 2, 4, TREE, false>), grid, dim3(256), 0, st, q, k, v, dm, out);
   }
   if (dm.n_split > 1) {
-    hipLaunchKernelGGL((paged_attn_join<D>), dim3((unsigned)((out.n_rows + 3) / 4)), dim3(256), 0, st, out, dm.n_split, dm.c2);
+    hipLaunchKernelGGL((paged_attn_join<D>), dim3((dm.T * dm.HQ + 3) / 4, dm.B), dim3(256), 0, st, dm, out);
   }
   return HILS_OK;
 }
@@ -1049,6 +1107,7 @@ extern "C" int hils_paged_attn(const void* q, const void* k_pages, const void* v
   HILS_REQUIRE(need == 0 || (workspace && workspace_bytes >= need),
                "hils_paged_attn: workspace too short: %zu bytes, %zu needed", workspace_bytes, need);
   PagedDims dm{B, T, HQ, H, HQ / H, window, expand_to_chunk, mask_lmk, max_pages, num_pages, seq_len, pl.n_blk, pl.n_split,
+               lengths && pl.n_split > 1 && B > 1 && B <= 64,
                parents_per_batch ? T : 0, hils_udiv_magic(HQ / H), sm_scale * HILS_LOG2E, (long)q_batch_stride,
                (long)q_token_stride, (long)q_head_stride, page_table, lengths, parents};
   PagedOut out{(bf16_t*)o, lse, (float*)workspace, rows};
