@@ -553,24 +553,26 @@ paged_attn_rows(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, cons
 }
 
 // ---- many rows ---------------------------------------------------------------------------------
-// 32 rows a wavefront; pages go straight into LDS, keys into one of four buffers, values into one of four others, asked for
-// three steps before they are used.  32x32x16 products: a row's scores of half a page (32 tokens) are 16 registers of two
+// 32 rows a wavefront, or two wavefronts that have half of every page each and add up at the end (KW == 2: where the rows fill
+// less than half of a compute unit's wavefronts; trees of 64 tokens for 4 sequences, 8 KV heads of 128, window 512: 64 rows by
+// 4 wavefronts 15.9 us, by 2 17.9); pages go straight into LDS, keys into one of four buffers, values into one of four others,
+// asked for two or three steps before they are used.  32x32x16 products: a row's scores of half a page (32 tokens) are 16 registers of two
 // lanes, which are the second product's operand as they are.  A step issues, half by half, the products of page p's output
 // and of page p + 1's scores between the exponentials of the half page behind (the matrix and vector instructions of one
 // wavefront overlap, those of two that run in step hardly do).  The exponentials' reference point follows a row's maximum
 // only when a score is more than 2^6 above it: the others need no reduction over lanes and no rescaling, and probabilities
 // of up to 2^6 enter sum and output alike.
 // The buffers come first: their places are then plain offsets, and a buffer's number is two bits of them.
-template <int D, int NW, bool TREE>
+template <int D, int NW, int KW, bool TREE>
 static constexpr size_t paged_tiles_smem() {
-  return 2 * 4 * (size_t)PA_PAGE * 2 * D + (TREE ? (NW * 32 * (PA_WORDS + 1) + PA_MAX_TREE) * sizeof(int) : 0);
+  return 2 * 4 * (size_t)PA_PAGE * 2 * D + (TREE ? (NW / KW * 32 * (PA_WORDS + 1) + PA_MAX_TREE) * sizeof(int) : 0);
 }
 
-template <int D, int NW, bool TREE>
+template <int D, int NW, int KW, bool TREE>
 __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)))
 paged_attn_tiles(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, const bf16_t* __restrict__ v, PagedDims dm,
                  PagedOut out) {
-  constexpr int NT = NW * 64, ROWS = NW * 32, KS = D / 16, FT = D / 32, RP = 2 * D, SEG = D / 8;
+  constexpr int NT = NW * 64, RW = NW / KW, ROWS = RW * 32, KS = D / 16, FT = D / 32, RP = 2 * D, SEG = D / 8;
   constexpr int NB = 4, PAGE = PA_PAGE * RP, NP = PAGE / 1024 / NW;  // loads of a page's keys per wavefront
   static_assert(NP >= 1 && NP * NW * 1024 == PAGE, "every wavefront loads whole rows");
   constexpr float LAZY = 6.f;
@@ -581,6 +583,7 @@ paged_attn_tiles(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, con
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, h = lane >> 5;
+  const int rg = wave % RW, kg = wave / RW;  // rows and half of every page (KW == 2) that are this wavefront's
   PagedUnit at;
   if (!paged_unit(dm, lane, at)) return;
   const int blk = at.blk, hk = at.hk, b = at.b;
@@ -629,7 +632,7 @@ paged_attn_tiles(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, con
     for (int i = 0; i < NP; ++i) lz_dma16(to + i * 1024, d_off[i & 3], from + (i >> 2) * 4096);
   };
 
-  const int r = r0 + wave * 32 + col;
+  const int r = r0 + rg * 32 + col;
   const int rc = r < r1 ? r : r1 - 1;
   const int my_t = hils_udiv(rc, dm.G, dm.g_magic), my_g = rc - my_t * dm.G;
   const bool live = r < r1 && sp.alive;
@@ -650,6 +653,7 @@ paged_attn_tiles(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, con
   if constexpr (TREE) asm volatile("" : "+v"(par[0]), "+v"(par[(PA_MAX_TREE - 1) / NT]));
   const unsigned long long place0 = page_place(0), place1 = page_place(1), place2 = page_place(2);
   unsigned long long place = page_place(3);  // of page x + 3 before step x
+  unsigned long long place_k = KW == 2 ? page_place(4) : 0;  // of page x + 4
   if (n > 0) {
     fetch(k_pool + place0, k_buffer(0));
     fetch(k_pool + place1, k_buffer(1));
@@ -696,13 +700,13 @@ paged_attn_tiles(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, con
   float ref = HILS_NEG_INF, l_run = 0.f;  // reference point (log2 units) and this lane's share of the sum
   unsigned k_off[KS], v_off[FT][2];       // this lane's places in a half page, in the buffers of this step
 #pragma unroll
-  for (int ks = 0; ks < KS; ++ks) k_off[ks] = (unsigned)(col * RP + ((2 * ks + h) ^ lz_swz<D>(col)) * 16);
+  for (int ks = 0; ks < KS; ++ks) k_off[ks] = (unsigned)((col + 32 * kg) * RP + ((2 * ks + h) ^ lz_swz<D>(col)) * 16);
 #pragma unroll
   for (int ft = 0; ft < FT; ++ft)
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int row = 4 * h + 8 * e + ((lane & 15) >> 2), pc = ft * 4 + (lane >> 4 & 1) * 2 + (lane >> 1 & 1);
-      v_off[ft][e] = (unsigned)(NB * PAGE + row * RP + (pc ^ lz_swz<D>(row)) * 16 + (lane & 1) * 8);
+      v_off[ft][e] = (unsigned)(NB * PAGE + (row + 32 * kg) * RP + (pc ^ lz_swz<D>(row)) * 16 + (lane & 1) * 8);
     }
 
   auto products = [&](f32x16_t& st, int half) __attribute__((always_inline)) {
@@ -769,15 +773,18 @@ paged_attn_tiles(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, con
   };
   f32x16_t sa, sb;  // scores of first halves, of second halves
   pa_u4 pa[2], pb[2];
-  static_assert(NP <= KS, "half a step issues the loads of a page's keys or values");
+  static_assert(KW * NP <= KS, "a half page's products issue the loads of a page's keys or values, or both");
   constexpr int AH = 3;  // products of each kind that operands are read ahead of
-  // Step x: the products of page x's output and of page x + 1's scores, a pair of them at a time (D / 16 pairs a half), and
-  // between them the probabilities of the half page behind, from the scores that the half step before has left; the loads of
-  // page x + 3's values and x + 4's keys.
-  auto step = [&](int x, unsigned long long v_from, unsigned v_to, unsigned long long k_from, unsigned k_to) __attribute__((always_inline)) {
+  // Step x, both halves of a page a wavefront's: the products of page x's output and of page x + 1's scores, a pair of them at
+  // a time (D / 16 pairs a half), and between them the probabilities of the half page behind, from the scores that the half
+  // step before has left; the loads of page x + 3's values and x + 4's keys.  One half a wavefront's (KW == 2): the products of
+  // page x's output and of page x + 2's scores, between them the probabilities of page x + 1; the loads of page x + 3's values
+  // and x + 5's keys.
+  auto step = [&](int x, unsigned long long v_from, unsigned v_to, unsigned long long k_from, unsigned k_to, f32x16_t& s1,
+                  f32x16_t& s2, pa_u4 (&p1)[2], pa_u4 (&p2)[2]) __attribute__((always_inline)) {
     bf16x8_t va[AH + 1], ka[AH + 1];
     auto operands = [&](int y) __attribute__((always_inline)) {
-      const int half = y / KS, s = y % KS / FT, ft = y % FT;
+      const int half = y / KS, s = y % KS / FT, ft = y % FT;  // (KW == 2: the half is in the offsets)
       const unsigned char* a0p = pa_dyn + (v_off[ft][0] + (half * 32 + s * 16) * RP);
       const unsigned char* a1p = pa_dyn + (v_off[ft][1] + (half * 32 + s * 16) * RP);
       const pa_s4 a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) pa_s4*)a0p);
@@ -789,10 +796,11 @@ paged_attn_tiles(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, con
     // the y-th pair; probabilities of `now` into pn
     auto pair = [&](auto yc, f32x16_t& now, f32x16_t& nx, const pa_u4 (&p)[2], pa_u4 (&pn)[2]) __attribute__((always_inline)) {
       constexpr int y = decltype(yc)::value, z = y % KS;
-      if constexpr (y + AH < 2 * KS) operands(y + AH);
+      if constexpr (y + AH < 2 / KW * KS) operands(y + AH);
       acc[y % FT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va[y % (AH + 1)], __builtin_bit_cast(bf16x8_t, p[z / FT]), acc[y % FT], 0, 0, 0);
       nx = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka[y % (AH + 1)], qa[z], nx, 0, 0, 0);
-      if constexpr (z < NP) lz_dma16((y < KS ? v_to : k_to) + z * 1024, d_off[z & 3], (y < KS ? v_from : k_from) + (z >> 2) * 4096);
+      if constexpr (KW == 2 && z >= NP && z < 2 * NP) lz_dma16(k_to + (z - NP) * 1024, d_off[(z - NP) & 3], k_from + ((z - NP) >> 2) * 4096);
+      else if constexpr (z < NP) lz_dma16((y < KS ? v_to : k_to) + z * 1024, d_off[z & 3], (y < KS ? v_from : k_from) + (z >> 2) * 4096);
       if (z > 0) {  // (none beside the first pair: its scores are not there yet)
         constexpr int per = KS == 8 ? 2 : 4, first = (z - 1) * per;
         weigh(now, pn, sum, std::integral_constant<int, first>{}, std::integral_constant<int, z == KS - 1 ? 16 - first : per>{});
@@ -829,29 +837,42 @@ paged_attn_tiles(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, con
 #pragma unroll
     for (int y = 0; y < AH; ++y) operands(y);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) sa[i] = 0.f;
+    for (int i = 0; i < 16; ++i) s2[i] = 0.f;
     sum[0] = sum[1] = 0.f;
     __builtin_amdgcn_sched_barrier(0);
-    PA_PAIR(0, sb, sa, pa, pb);
-    hide(sb, x, 1, 4);
-    asm volatile("" : "+v"(sb));  // (the exponentials stay behind this point, between the products)
+    PA_PAIR(0, s1, s2, p1, p2);
+    if (KW == 2) hide(s1, x + 1, kg, 4);
+    else hide(s1, x, 1, 4);
+    asm volatile("" : "+v"(s1));  // (the exponentials stay behind this point, between the products)
     __builtin_amdgcn_sched_barrier(0);
-    PA_HALF(0, sb, sa, pa, pb)
-    finish(sb, pb);
+    PA_HALF(0, s1, s2, p1, p2)
+    finish(s1, p2);
+    if constexpr (KW == 1) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) sb[i] = 0.f;
-    sum[0] = sum[1] = 0.f;
-    __builtin_amdgcn_sched_barrier(0);
-    PA_PAIR(KS, sa, sb, pb, pa);
-    hide(sa, x + 1, 0, 3);
-    asm volatile("" : "+v"(sa));
-    __builtin_amdgcn_sched_barrier(0);
-    PA_HALF(KS, sa, sb, pb, pa)
-    finish(sa, pa);
+      for (int i = 0; i < 16; ++i) s1[i] = 0.f;
+      sum[0] = sum[1] = 0.f;
+      __builtin_amdgcn_sched_barrier(0);
+      PA_PAIR(KS, s2, s1, p2, p1);
+      hide(s2, x + 1, 0, 3);
+      asm volatile("" : "+v"(s2));
+      __builtin_amdgcn_sched_barrier(0);
+      PA_HALF(KS, s2, s1, p2, p1)
+      finish(s2, p1);
+    }
 #undef PA_HALF
 #undef PA_PAIR
   };
-  if (n > 0) {
+  auto turn_k = [&](int x) __attribute__((always_inline)) {  // the bit in which the buffers of pages x and x + 1 differ
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) k_off[ks] ^= x & 1 ? 2 * PAGE : PAGE;
+  };
+  auto turn_v = [&](int x) __attribute__((always_inline)) {
+#pragma unroll
+    for (int ft = 0; ft < FT; ++ft)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) v_off[ft][e] ^= x & 1 ? 2 * PAGE : PAGE;
+  };
+  if (KW == 1 && n > 0) {
     lz_landed<6 * NP>();  // keys of page 0
     lds_barrier();
     products(sa, 0);
@@ -863,16 +884,67 @@ paged_attn_tiles(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, con
       lds_barrier();        // ... of all wavefronts; keys of x and values of x - 1 have been read
       const unsigned long long v_from = v_pool + place;
       place = page_place(x + 4);
-      const unsigned other = x & 1 ? 2 * PAGE : PAGE;  // the bit in which the buffers of pages x and x + 1 differ
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) k_off[ks] ^= other;
-      step(x, v_from, v_buffer(x + 3), k_pool + place, k_buffer(x + 4));
+      turn_k(x);
+      step(x, v_from, v_buffer(x + 3), k_pool + place, k_buffer(x + 4), sb, sa, pa, pb);
+      turn_v(x);
+    }
+    lz_landed<0>();
+  }
+  if (KW == 2 && n > 0) {
+    lz_landed<5 * NP>();  // keys of pages 0 and 1
+    lds_barrier();
+    products(sa, 0);
+    turn_k(0);
+    products(sb, 0);
+    hide(sa, 0, kg, 4);
+    (void)settle(sa, pa, highest(sa));
+    lz_landed<3 * NP>();
+    lds_barrier();  // (the keys of page 0 have been read)
+    fetch(k_pool + place_k, k_buffer(4));
+    auto one = [&](int x, f32x16_t& s1, f32x16_t& s2, pa_u4 (&p1)[2], pa_u4 (&p2)[2]) __attribute__((always_inline)) {
+      lz_landed<4 * NP>();  // keys of x + 2, values of x
+      lds_barrier();        // ... of all wavefronts; keys of x + 1 and values of x - 1 have been read
+      const unsigned long long v_from = v_pool + place;
+      place = place_k;
+      place_k = page_place(x + 5);
+      turn_k(x + 1);
+      step(x, v_from, v_buffer(x + 3), k_pool + place_k, k_buffer(x + 5), s1, s2, p1, p2);
+      turn_v(x);
+    };
+    for (int x = 0; x < n; x += 2) {
+      one(x, sb, sa, pa, pb);
+      if (x + 1 < n) one(x + 1, sa, sb, pb, pa);
+    }
+    lz_landed<0>();
+  }
+  if constexpr (KW == 2) {  // the halves' results meet in the buffers
+    float* const mine = (float*)pa_dyn + rg * (FT * 16 + 2) * 64 + lane * 4;
+    float* const mine_l = (float*)pa_dyn + rg * (FT * 16 + 2) * 64 + FT * 16 * 64 + lane;
+    lds_barrier();
+    if (kg == 1) {
 #pragma unroll
       for (int ft = 0; ft < FT; ++ft)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) v_off[ft][e] ^= other;
+        for (int i4 = 0; i4 < 4; ++i4)
+          *(f32x4_t*)(mine + (ft * 4 + i4) * 256) = f32x4_t{acc[ft][4 * i4], acc[ft][4 * i4 + 1], acc[ft][4 * i4 + 2], acc[ft][4 * i4 + 3]};
+      mine_l[0] = ref;
+      mine_l[64] = l_run;
     }
-    lz_landed<0>();
+    lds_barrier();
+    if (kg == 1) return;
+    const float ref1 = mine_l[0], to = fmaxf(ref, ref1);
+    // (neither has a finite score: the sums are zero, or scores that are not numbers, which the sums keep)
+    const float f0 = to > HILS_NEG_INF ? __builtin_amdgcn_exp2f(ref - to) : 1.f, f1 = to > HILS_NEG_INF ? __builtin_amdgcn_exp2f(ref1 - to) : 1.f;
+#pragma unroll
+    for (int ft = 0; ft < FT; ++ft)
+#pragma unroll
+      for (int i4 = 0; i4 < 4; ++i4) {
+        const f32x4_t x = *(const f32x4_t*)(mine + (ft * 4 + i4) * 256);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[ft][4 * i4 + i] = fmaf(acc[ft][4 * i4 + i], f0, x[i] * f1);
+      }
+    l_run = fmaf(l_run, f0, mine_l[64] * f1);
+    ref = to;
   }
 
   // accumulator register i of tile ft is feature ft*32 + (i >> 2)*8 + 4h + (i & 3) of row `col`
@@ -901,7 +973,7 @@ paged_attn_tiles(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, con
     while (odd) {
       const int i = __builtin_ctzll(odd);
       odd &= odd - 1;
-      const int rr = r0 + wave * 32 + i, tr = hils_udiv(rr, dm.G, dm.g_magic), gr = rr - tr * dm.G;
+      const int rr = r0 + rg * 32 + i, tr = hils_udiv(rr, dm.G, dm.g_magic), gr = rr - tr * dm.G;
       const int left = TREE ? left_s[tr - t0] : paged_left(sp.base + tr, dm);
       paged_redo_row<D>(dm, out, q + b * dm.q_sb + tr * dm.q_st + (hk * dm.G + gr) * dm.q_sh, k, v, table, hk, sp.base, sp.p0,
                         sp.p1, tr, left, TREE ? mask_s + (tr - t0) * PA_WORDS : nullptr,
@@ -969,27 +1041,29 @@ __global__ void __launch_bounds__(256) paged_attn_join(PagedDims dm, PagedOut ou
 
 // ---- host ----------------------------------------------------------------------------------------
 struct PagedPlan {
-  bool tiles, past;            // past: values are read past the caches
-  int nr, nw, n_blk, n_split;  // 16 nr rows a workgroup, or 32 nw
+  bool past;           // values are read past the caches
+  int rows, nw, kw;    // rows a workgroup; wavefronts of the tile kernel and those that share a row (0: the row kernel)
+  int n_blk, n_split;
 };
 
 // Which kernel, and over how many workgroups a range of keys is split.
 // What the variants cost, in microseconds, from sweeps of every variant and share count over 1 to 32 sequences, 1 to 128 new
 // tokens, windows of 512 tokens and contexts of 512 to 32768: a launch is about
 //   fixed + rounds * (start + page * pages of a share)
-// or, where that is longer, the bytes read once at 6.4 TB/s; a round is one workgroup on every compute unit, and where a second
-// one fits beside it (heads of 64) the two take (1 + beside) rounds.  More than one share adds the join.  The choice that this
-// predicts to be shortest was within 2 % of the best measured one on average and within 15 % in the worst of 82 calls; fixed
+// or, where that is longer, the bytes read once at 6.8 TB/s or those that all workgroups read at 21 TB/s; a round is one
+// workgroup on every compute unit, and where a second one fits beside it (heads of 64) the two take (1 + beside) rounds.  More
+// than one share adds the join, its results written and read at 3.2 TB/s.  The choice that this predicts to be shortest was
+// within 2 % of the best measured one on average and within 17 % in the worst of 159 calls; fixed
 // thresholds on rows and pages were 15 % off on average and lost up to 1.7 times (1 token, 8 KV heads of 128, 4096 tokens: 8
 // shares 12.9 us, 32 shares 8.5; 16 tokens, 2 KV heads of 64, window 512: 32 rows a workgroup 10.1, 16 rows 7.5).
 struct PagedCost {
-  int tiles, n;  // the tile kernel's wavefronts, or the row kernel's 16-row blocks
+  int rows, nw, kw;
   float fixed, start, page, beside;
 };
-static const PagedCost kPagedCost128[] = {{0, 1, 1.9f, 3.4f, 0.59f, 1.f}, {0, 2, 3.2f, 4.0f, 0.76f, 1.f}, {1, 2, 3.7f, 2.5f, 1.11f, 1.f},
-                                          {1, 4, 4.4f, 2.4f, 1.18f, 1.f}, {1, 8, 3.1f, 4.0f, 1.59f, 1.f}};
-static const PagedCost kPagedCost64[] = {{0, 1, 3.3f, 1.4f, 0.28f, 1.f}, {0, 2, 4.3f, 1.5f, 0.48f, 0.4f}, {1, 2, 3.7f, 2.4f, 0.85f, 0.4f},
-                                         {1, 4, 4.9f, 1.8f, 0.88f, 0.5f}};
+static const PagedCost kPagedCost128[] = {{16, 0, 0, 1.8f, 4.0f, 0.56f, 1.f}, {32, 0, 0, 3.5f, 4.0f, 0.73f, 1.f}, {64, 4, 2, 4.8f, 2.7f, 0.76f, 1.f},
+                                          {128, 8, 2, 6.0f, 2.8f, 0.95f, 1.f}, {256, 8, 1, 6.9f, 0.3f, 1.60f, 1.f}};
+static const PagedCost kPagedCost64[] = {{16, 0, 0, 2.8f, 1.9f, 0.28f, 0.94f}, {32, 0, 0, 3.6f, 2.1f, 0.48f, 0.42f}, {64, 4, 2, 4.1f, 2.7f, 0.57f, 0.38f},
+                                         {128, 4, 1, 6.9f, 0.f, 0.89f, 0.49f}};
 
 static PagedPlan paged_choose(int B, int T, int HQ, int H, int D, int window, int max_pages) {
   PagedPlan best = {};
@@ -999,12 +1073,12 @@ static PagedPlan paged_choose(int B, int T, int HQ, int H, int D, int window, in
     const long pages = ((long)window + tokens + 2 * PA_PAGE - 3) / PA_PAGE;
     return pages < max_pages ? pages : max_pages;
   };
-  const float read = (float)B * H * pages_of(T) * PA_PAGE * D * 4 / 6.4e6f;
+  const float read = (float)B * H * pages_of(T) * PA_PAGE * D * 4 / 6.8e6f;
   float least = 0.f;
   const PagedCost* cost = D == 128 ? kPagedCost128 : kPagedCost64;
   for (int i = 0; i < (D == 128 ? 5 : 4); ++i) {
     const PagedCost& c = cost[i];
-    const int per = c.tiles ? 32 * c.n : 16 * c.n;
+    const int per = c.rows;
     if (i && rows <= per / 2) break;  // (the variants before hold every row with fewer of them empty)
     const long n_blk = (rows + per - 1) / per, tokens = per / G + 1 > PA_MAX_TREE ? per / G + 1 : PA_MAX_TREE;
     const long pages = pages_of(T < tokens ? T : tokens);
@@ -1012,13 +1086,16 @@ static PagedPlan paged_choose(int B, int T, int HQ, int H, int D, int window, in
       const long n = (n_blk * n_split * H * B + cus - 1) / cus;
       const float rounds = c.beside < 1.f ? (n / 2) * (1.f + c.beside) + n % 2 : (float)n;
       const float work = rounds * (c.start + c.page * ((pages + n_split - 1) / n_split));
-      // (the fourth powers: a sweep near both bounds takes longer than either)
-      float t = c.fixed + sqrtf(sqrtf(work * work * work * work + read * read * read * read));
-      if (n_split > 1) t += 2.4f + (float)B * rows * H * n_split * (D + 2) * 8 / 3.7e6f;
+      const float near = (float)n_blk * n_split * H * B * ((pages + n_split - 1) / n_split) * PA_PAGE * D * 4 / 21e6f;
+      // (the fourth powers: a sweep near two bounds takes longer than either)
+      const auto fourth = [](float x) { return x * x * x * x; };
+      float t = c.fixed + sqrtf(sqrtf(fourth(work) + fourth(read) + fourth(near)));
+      if (n_split > 1) t += 2.9f + (float)B * rows * H * n_split * (D + 2) * 8 / 3.2e6f;
       if (best.n_blk && t >= least) continue;
       least = t;
-      best.tiles = c.tiles;
-      best.nr = best.nw = c.n;
+      best.rows = c.rows;
+      best.nw = c.nw;
+      best.kw = c.kw;
       best.n_blk = (int)n_blk;
       best.n_split = n_split;
     }
@@ -1056,25 +1133,22 @@ template <int D, bool TREE>
 static int paged_launch(const PagedPlan& pl, const bf16_t* q, const bf16_t* k, const bf16_t* v, const PagedDims& dm,
                         const PagedOut& out, hipStream_t st) {
   const dim3 grid((unsigned)(((long)dm.n_blk * dm.n_split * dm.H * dm.B + 7) / 8 * 8));
-  if (pl.tiles) {
-#define PA_TILES(NW_)                                                                                                     \
-  do {                                                                                                                   \
-    static HilsLdsReserve reserved;                                                                                      \
-    constexpr size_t smem = paged_tiles_smem<D, NW_, TREE>();                                                            \
-    if (int rc = hils_reserve_lds(&reserved, (const void*)paged_attn_tiles<D, NW_, TREE>, smem, "hils_paged_attn")) return rc; \
-    hipLaunchKernelGGL((paged_attn_tiles<D, NW_, TREE>), grid, dim3(NW_ * 64), smem, st, q, k, v, dm, out);              \
+#define PA_TILES(NW_, KW_)                                                                           \
+  do {                                                                                               \
+    static HilsLdsReserve reserved;                                                                  \
+    const auto kern = paged_attn_tiles<D, NW_, KW_, TREE>;                                           \
+    constexpr size_t smem = paged_tiles_smem<D, NW_, KW_, TREE>();                                   \
+    if (int rc = hils_reserve_lds(&reserved, (const void*)kern, smem, "hils_paged_attn")) return rc; \
+    hipLaunchKernelGGL(kern, grid, dim3(NW_ * 64), smem, st, q, k, v, dm, out);                      \
   } while (0)
-    if constexpr (D == 128) {
-      if (pl.nw == 8) PA_TILES(8);
-    }
-    if (pl.nw == 4) PA_TILES(4);
-    if (pl.nw == 2) PA_TILES(2);
+  if (pl.rows == 16 && pl.past) hipLaunchKernelGGL((paged_attn_rows<D, 1, 8, TREE, true>), grid, dim3(512), 0, st, q, k, v, dm, out);
+  else if (pl.rows == 16) hipLaunchKernelGGL((paged_attn_rows<D, 1, 8, TREE, false>), grid, dim3(512), 0, st, q, k, v, dm, out);
+  else if (pl.rows == 32) hipLaunchKernelGGL((paged_attn_rows<D, 2, 4, TREE, false>), grid, dim3(256), 0, st, q, k, v, dm, out);
+  else if (pl.rows == 64) PA_TILES(4, 2);
+  else if constexpr (D == 64) PA_TILES(4, 1);
+  else if (pl.rows == 128) PA_TILES(8, 2);
+  else PA_TILES(8, 1);
 #undef PA_TILES
-  } else {
-    if (pl.nr == 1 && pl.past) hipLaunchKernelGGL((paged_attn_rows<D, 1, 8, TREE, true>), grid, dim3(512), 0, st, q, k, v, dm, out);
-    else if (pl.nr == 1) hipLaunchKernelGGL((paged_attn_rows<D, 1, 8, TREE, false>), grid, dim3(512), 0, st, q, k, v, dm, out);
-    else hipLaunchKernelGGL((paged_attn_rows<D, 2, 4, TREE, false>), grid, dim3(256), 0, st, q, k, v, dm, out);
-  }
   if (dm.n_split > 1) {
     hipLaunchKernelGGL((paged_attn_join<D>), dim3((dm.T * dm.HQ + 3) / 4, dm.B), dim3(256), 0, st, dm, out);
   }

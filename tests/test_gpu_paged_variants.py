@@ -14,7 +14,9 @@ CASES = [(32, 8, 2, 64, 512, 1024), (32, 8, 8, 33, 1 << 20, 900), (32, 8, 8, 64,
          (4, 4, 5, 200, 1 << 20, 900), (6, 2, 5, 100, 1 << 20, 4500), (32, 8, 3, 33, 1 << 20, 4500), (5, 1, 16, 33, 1 << 20, 4500),
          (32, 8, 1, 33, 1 << 20, 18000), (32, 8, 2, 33, 1 << 20, 9000), (4, 4, 1, 33, 1 << 20, 18000), (6, 2, 2, 33, 1 << 20, 18000),
          (5, 1, 2, 33, 1 << 20, 18000), (4, 4, 16, 33, 1 << 20, 18000), (32, 8, 16, 7, 1 << 20, 4500), (32, 8, 8, 7, 1 << 20, 18000),
-         (4, 4, 16, 1, 1 << 20, 18000), (5, 1, 1, 1, 1 << 20, 18000), (32, 8, 16, 40, 1 << 20, 9000), (32, 8, 16, 4, 1 << 20, 9000)]
+         (4, 4, 16, 1, 1 << 20, 18000), (5, 1, 1, 1, 1 << 20, 18000), (32, 8, 16, 40, 1 << 20, 9000), (32, 8, 16, 4, 1 << 20, 9000),
+         (32, 8, 1, 256, 512, 1024), (6, 2, 3, 7, 1 << 20, 18000), (4, 4, 5, 20, 1 << 20, 18000), (6, 2, 3, 33, 1 << 20, 18000),
+         (32, 8, 1, 100, 1 << 20, 4500), (32, 8, 2, 33, 1 << 20, 18000)]
 
 
 def _inputs(dev, D, HQ, H, B, T, ctx, tree, seed):
@@ -48,6 +50,19 @@ def test_sizes(pkg, dev, case, tree, D):
 
 
 @pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("case", [(8, 2, 2, 1000, 200, 2100), (6, 1, 1, 3001, 1 << 20, 3001), (32, 8, 3, 513, 512, 4500),
+                                  (4, 4, 2, 700, 1 << 20, 9000)], ids=str)
+def test_slices_of_a_prompt(pkg, dev, case, D):
+    HQ, H, B, T, window, ctx = case
+    note(f"paged attention of many tokens {case} D{D}")
+    q, k, v, table, lengths, _ = _inputs(dev, D, HQ, H, B, T, ctx, False, seed=T)
+    got = _call(pkg, q, k, v, table, lengths, window, None)
+    for b in range(B):
+        want = ref.attend_dense(q[b:b + 1], k, v, table[b:b + 1], lengths[b:b + 1], window)
+        ref.check_attention(tuple(x[b:b + 1] for x in got), want)
+
+
+@pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("tree", [False, True])
 @pytest.mark.parametrize("case", [(32, 8, 8, 64, 130, 1024), (32, 8, 5, 200, 1 << 20, 900), (16, 1, 16, 33, 1 << 20, 900),
                                   (4, 4, 1, 33, 1 << 20, 18000), (32, 8, 2, 33, 1 << 20, 9000), (4, 4, 16, 33, 1 << 20, 4500)], ids=str)
@@ -74,6 +89,20 @@ def test_stale_numbers(pkg, dev, case, tree, D, bad):
     keep = T - 1 if tree else T
     for b, want in enumerate(wants):
         ref.check_attention((o[b:b + 1, :keep], lse[b:b + 1, :keep]), tuple(x[:, :keep] for x in want))
+
+
+def test_a_sequence_apart(pkg, dev):
+    """Lengths from none to all of the table in one batch, whose shares the sequences divide by their lengths."""
+    note("very uneven lengths")
+    for HQ, H, B, T, D, lens in ((32, 8, 3, 33, 128, [9000, 33, 40]), (16, 2, 64, 1, 64, [9000] + [0, 1, 64, 65, 130, 500, 7] * 9),
+                                 (8, 2, 65, 2, 64, [9000] + [2, 64, 3, 900] * 16), (4, 1, 2, 1, 128, [0, 0]),
+                                 (32, 4, 5, 64, 128, [70, 9000, 64, 8999, 4000]), (4, 1, 40, 3, 128, [9000] * 2 + [3] * 38)):
+        gen = torch.Generator().manual_seed(B)
+        k, v, table = ref.cache(gen, B, 141, H, D, dev)
+        q = torch.randn(B, T, HQ, D, generator=gen).bfloat16().to(dev)
+        lengths = torch.tensor(lens, dtype=torch.int32, device=dev)
+        got = _call(pkg, q, k, v, table, lengths, 1 << 20, None)
+        ref.check_attention(got, ref.attend_dense(q, k, v, table, lengths, 1 << 20))
 
 
 @pytest.mark.parametrize("D", [64, 128])
