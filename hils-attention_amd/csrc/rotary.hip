@@ -143,8 +143,9 @@ rotary_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, const 
     const double turns = p * (w * 0.15915494309189533577);  // 1 / (2 pi)
     double sn, cs;
     sincospi(2.0 * (turns - rint(turns)), &sn, &cs);
-    cos_s[i] = cs * dm.scale;
-    sin_s[i] = sn * dm.scale * dm.sign;
+    const int at = i ^ (i >> 4 & 2);  // (eight units in step read angles 64 bytes apart: of two that share banks one reads ahead)
+    cos_s[at] = cs * dm.scale;
+    sin_s[at] = sn * dm.scale * dm.sign;
   }
   __syncthreads();
   for (int e0 = tid; e0 < total; e0 += 256 * ROT_UN) {
@@ -153,8 +154,13 @@ rotary_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, const 
     for (int x = 0; x < ROT_UN; ++x) {
       if (!to[x]) continue;
       if (tab[x] >= 0) {
-        const double* c = cos_s + tab[x];
-        const double* sn = sin_s + tab[x];
+        double c[8], sn[8];
+        const int turn = tab[x] >> 4 & 2;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          c[i] = cos_s[(tab[x] + (i & 6) ^ turn) + (i & 1)];
+          sn[i] = sin_s[(tab[x] + (i & 6) ^ turn) + (i & 1)];
+        }
         const uint4 l0 = lo[x], h0 = hi[x];
         rotary_turn<INTERLEAVED>(l0, h0, c, sn, lo[x], hi[x]);
       }
