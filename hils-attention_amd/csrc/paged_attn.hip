@@ -1175,7 +1175,7 @@ extern "C" int hils_paged_attn(const void* q, const void* k_pages, const void* v
   HILS_REQUIRE(max_pages <= (1 << 24), "hils_paged_attn: the page table is too wide");
   HILS_REQUIRE(lengths || (seq_len >= T && seq_len <= (long)max_pages * PA_PAGE),
                "hils_paged_attn: seq_len %d is shorter than the %d tokens or longer than the page table", seq_len, T);
-  HILS_REQUIRE(B <= 65535 && H <= 65535 && (long)T * (HQ / H) * (HQ / H) < (1l << 31), "hils_paged_attn: sizes too large for the grid");
+  HILS_REQUIRE(B <= 65535 && H <= 65535 && (long)T * (HQ / H) * (HQ / H) < (1l << 31) && (long)T * HQ < (1l << 31) - 4, "hils_paged_attn: sizes too large for the grid");
   HILS_REQUIRE(q_batch_stride % 8 == 0 && q_token_stride % 8 == 0 && q_head_stride % 8 == 0 && (uintptr_t)q % 16 == 0,
                "hils_paged_attn: q's strides and address must be multiples of 16 bytes");
   const PagedPlan pl = paged_plan(B, T, HQ, H, D, window, max_pages);

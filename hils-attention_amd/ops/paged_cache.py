@@ -48,8 +48,8 @@ def paged_flex_attn(q, k_pages, v_pages, page_table, seq_len, window_size, paren
     and those that follow them, see nothing (padding).  Without ``parents`` the tokens are a chain.  T <= 256 for a tree.
     Returns o (B,T,H_q,D) bf16 and lse (B,T,H_q) fp32, natural log; rows that see nothing: 0 and -inf."""
     args = (q, k_pages, v_pages, page_table, seq_len, int(window_size), parents, bool(mask_lmk), bool(expand_to_chunk), sm_scale)
-    if q.requires_grad:
-        return _inference("paged_flex_attn", lambda: _cabi.host().paged_flex_attn(*args), q)
+    if q.requires_grad or k_pages.requires_grad or v_pages.requires_grad:
+        return _inference("paged_flex_attn", lambda: _cabi.host().paged_flex_attn(*args), q, k_pages, v_pages)
     return _cabi.host().paged_flex_attn(*args)
 
 
@@ -64,7 +64,7 @@ def copy_pages(pools, src, dst):
     """``pool[dst[i]] = pool[src[i]]`` for every i and every pool, in one launch.  ``pools``: up to eight contiguous tensors
     with the same number of pages (first dimension), any types.  ``src``, ``dst``: int32 or int64 vectors on the GPU, or
     sequences of ints.  Pairs with an index out of range are left out.  A page that is written must be in no other pair:
-    checked for sequences, the caller's duty for tensors on the GPU (the result is one of the pages that meet there)."""
+    checked for sequences, the caller's duty for tensors on the GPU (pieces of the pages that meet there are mixed)."""
     pools = list(pools)
     if not isinstance(src, torch.Tensor) or not isinstance(dst, torch.Tensor):
         src, dst = [int(x) for x in src], [int(x) for x in dst]

@@ -311,19 +311,18 @@ class HiLSPagedLayer:
 
     def _own_tail(self, tokens):
         """Before a write behind ``tokens`` tokens: copies of the partly filled pages that other sequences use too."""
-        c = tokens // self.S
-        src, dst, who = [], [], []
-        for b in self._tail_sharers(tokens):
-            page = self._pages[b][c]
-            new = self.free_pages.pop()
+        c, who = tokens // self.S, self._tail_sharers(tokens)
+        if not who:
+            return
+        src, dst = [self._pages[b][c] for b in who], self.free_pages[-len(who):]
+        copy_pages(self._pools(), src, dst)
+        dev = self.page_table.device
+        self.page_table[torch.tensor(who, device=dev), c] = torch.tensor(dst, dtype=torch.int32, device=dev)
+        del self.free_pages[-len(who):]
+        for b, page, new in zip(who, src, dst):
             self._users[page] -= 1
             self._users[new] = 1
             self._pages[b][c] = new
-            src.append(page), dst.append(new), who.append(b)
-        if src:
-            copy_pages(self._pools(), src, dst)
-            dev = self.page_table.device
-            self.page_table[torch.tensor(who, device=dev), c] = torch.tensor(dst, dtype=torch.int32, device=dev)
 
     def _tail_sharers(self, tokens):
         """The sequences that need a copy of their partly filled page: of its users all but the last."""
@@ -349,6 +348,15 @@ class HiLSPagedLayer:
         if copies:
             self._own_tail(a)
         self._take(have, need)
+        try:
+            return self._write(key_states, value_states, q, rotary, a, b_end)
+        except BaseException:  # (refused: the sequences are as they were)
+            self._keep_pages(a)
+            raise
+
+    def _write(self, key_states, value_states, q, rotary, a, b_end):
+        B, T, H, D = key_states.shape
+        S = self.S
         if self.k_pages.is_cuda and self.k_pages.dtype == torch.bfloat16 and D % 16 == 0 and D <= 1024:
             return paged_append(key_states, value_states, self.k_pages, self.v_pages, self.page_table, b_end, q=q, **rotary)
         # a cache in a type that the attention does not take is kept all the same
@@ -360,6 +368,22 @@ class HiLSPagedLayer:
         self.k_pages[pages, hh, slots] = key_states
         self.v_pages[pages, hh, slots] = value_states
         return None
+
+    def _check_prior(self, tokens, mu_q):
+        """Refuse prior queries that do not go with the chunks that `tokens` tokens complete (before anything is changed)."""
+        n, c0 = tokens // self.S - self.pooled_chunks, self.pooled_chunks
+        if n <= 0:
+            return
+        if mu_q is None:
+            assert not self.has_prior, "this cache keeps a prior bias: update() needs mu_q for new chunks"
+            assert self.h_lmk == self.H, (
+                "a layer built without chunk pooling keeps the attention pool's keys: update() needs mu_q")
+            return
+        assert mu_q.dim() == 4 and (mu_q.shape[0], mu_q.shape[1], mu_q.shape[3]) == (self.B, n, self.D), (
+            f"mu_q shape {tuple(mu_q.shape)}")
+        assert self.prior_pages is not None, "construct the layer with num_q_heads to keep a prior bias"
+        assert mu_q.shape[2] == self.prior_pages.shape[1], f"mu_q shape {tuple(mu_q.shape)}"
+        assert c0 == 0 or self.has_prior, "the prior bias must be kept from the first chunk on"
 
     def _pool_full_chunks(self, mu_q):
         """Chunk keys (and the prior bias) of the chunks that are full and have none yet."""
@@ -378,20 +402,12 @@ class HiLSPagedLayer:
         if mu_q is not None:
             hq = mu_q.shape[2]
             G = hq // H
-            assert mu_q.shape == (B, n, hq, D), f"mu_q shape {tuple(mu_q.shape)}"
-            assert self.prior_pages is not None, "construct the layer with num_q_heads to keep a prior bias"
-            assert c0 == 0 or self.has_prior, "the prior bias must be kept from the first chunk on"
             lk, lb = _attention_pooled(mu_q.reshape(-1, 1, hq, D), kk.permute(0, 2, 1, 3).unsqueeze(1), H)
             self.prior_pages[pg] = lb.reshape(-1, hq)
             self.prior_hm[:, :, c0:full] = lb.view(B, n, H, G).permute(0, 2, 1, 3)
             self.has_prior = True
             if pooled is None:
-                assert hq == self.h_lmk, "attention-pooled chunk keys are per query head"
                 pooled = lk.reshape(-1, hq, D)
-        else:
-            assert not self.has_prior, "this cache keeps a prior bias: update() needs mu_q for new chunks"
-        assert pooled.shape[1] == self.h_lmk, (
-            "a layer built without chunk pooling keeps the attention pool's keys: update() needs mu_q")
         pooled = pooled.to(self.lmk_pages.dtype)
         self.lmk_pages[pg] = pooled
         self.lmk_hm[:, :, c0:full] = pooled.view(B, n, self.h_lmk, D).permute(0, 2, 1, 3)
@@ -406,6 +422,7 @@ class HiLSPagedLayer:
         ``paged_append``) the keys, and the queries ``q`` if given, are rotated on the way; returns the
         rotated q."""
         assert not self.drafted, "tokens are on trial: accept() first"
+        self._check_prior(self.seq_len + key_states.shape[1], mu_q)
         q = self._append(key_states, value_states, q, rotary)
         self.seq_len += key_states.shape[1]
         self._pool_full_chunks(mu_q)
@@ -460,6 +477,7 @@ class HiLSPagedLayer:
             up = list(range(-1, T - 1)) if self._parents is None else self._parents[b % len(self._parents)]
             if any(not 0 <= t < T for t in way) or any(up[t] != p for t, p in zip(way, [-1] + way)):
                 raise ValueError(f"accept: {way} is no way down the tree of sequence {b}")
+        self._check_prior(self.seq_len + n, mu_q)
         if n and not torch.equal(path, torch.arange(n).expand(self.B, n)):
             paged_accept(self.k_pages, self.v_pages, self.page_table, self.seq_len,
                          path.to(self.k_pages.device, torch.int32))

@@ -238,3 +238,48 @@ def test_layer_refusals(pkg, dev):
     c.draft(z(70), z(70))
     with pytest.raises(ValueError, match="too deep"):
         c.hils_attend(z(70, 4), torch.zeros(B, 70, 4, device=dev), 1, 16)
+
+
+def test_a_refused_call_changes_nothing(pkg, dev):
+    """A call that is refused after pages were mapped for it, or for its prior queries, leaves the sequences as they were."""
+    note("refused appends and acceptances")
+    B, H, HQ, D = 2, 2, 4, 64
+    gen = torch.Generator().manual_seed(4)
+    r = lambda t, h=H: torch.randn(B, t, h, D, generator=gen).bfloat16().to(dev)
+    a = _layer(pkg, dev, B, H, HQ, D, num_q_heads=HQ)
+    b = _layer(pkg, dev, B, H, HQ, D, num_q_heads=HQ)
+    k, v, mu = r(100), r(100), torch.randn(B, 1, HQ, D, generator=gen).bfloat16().to(dev)
+    for c in (a, b):
+        c.update(k, v, mu_q=mu)
+        c.fork([0, 0])
+    k, v, mu = r(70), r(70), torch.randn(B, 1, HQ, D, generator=gen).bfloat16().to(dev)
+    for call, kind in ((lambda: a.update(k, v, mu_q=mu, q=r(70, HQ)), AssertionError),      # q without frequencies
+                       (lambda: a.update(k.float(), v.float(), mu_q=mu), TypeError),
+                       (lambda: a.update(k, v), AssertionError),                            # no prior queries for a chunk
+                       (lambda: a.update(k, v, mu_q=mu[:, :, :2]), AssertionError),
+                       (lambda: a.draft(k, v, q=r(70, HQ)), AssertionError),
+                       (lambda: a.draft(k, v[:, :3]), AssertionError)):
+        with pytest.raises(kind):
+            call()
+        _books(a)
+        assert a.seq_len == 100 and a.drafted == 0 and a.pooled_chunks == 1
+    for c in (a, b):
+        c.draft(k, v)
+    with pytest.raises(AssertionError, match="mu_q"):
+        a.accept(list(range(40)))
+    assert a.drafted == 70 and a.seq_len == 100
+    for c in (a, b):
+        c.accept(list(range(40)), mu_q=mu)
+        _books(c)
+    _same(a, b)
+    assert torch.equal(a.prior_hm, b.prior_hm) and a.pooled_chunks == 2
+
+
+def test_pages_that_want_gradients(pkg, dev):
+    note("no backward through the attention on pages")
+    gen = torch.Generator().manual_seed(1)
+    k, v, table = ref.cache(gen, 1, 2, 1, 64, dev)
+    q = torch.randn(1, 1, 2, 64, generator=gen).bfloat16().to(dev)
+    o, lse = pkg.paged_flex_attn(q, k.requires_grad_(), v, table, 100, 64)
+    with pytest.raises(RuntimeError, match="not supported"):
+        (o.float().sum() + lse.sum()).backward()
