@@ -457,7 +457,7 @@ paged_attn_rows(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, cons
   };
 
   {
-    // two units' loads in flight; past the last unit the same one is asked for again and not worked on
+    // two units' loads in flight (and none that are not worked on: a window's wavefronts have two or three units)
     pa_u4 ka[2][KS], va[VI], kc[2][KS], vc[VI];
     int n_mine = u1 > u0 + wave ? (u1 - u0 - wave + NWV - 1) / NWV : 0;
     auto page_at = [&](int i) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(pages_of, i & 63); };
@@ -491,16 +491,22 @@ paged_attn_rows(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, cons
       return page_at(i);
     };
     int u = u0 + wave, i = 0;
-    for (; i + 1 < n_mine; i += 2, u += 2 * NWV) {
+    for (; i + 2 < n_mine; i += 2, u += 2 * NWV) {
       pg_c = next_page(i + 1);
       issue(kc, vc, pg_c, (u + NWV) & 1);
       if ((unsigned)pg_a < (unsigned)dm.num_pages) unit(ka, va, u);
-      const bool more = i + 2 < n_mine;  // (else the last one is asked for again and not worked on)
-      pg_a = more ? next_page(i + 2) : pg_c;
-      issue(ka, va, pg_a, (more ? u : u + NWV) & 1);
+      pg_a = next_page(i + 2);
+      issue(ka, va, pg_a, u & 1);
       if ((unsigned)pg_c < (unsigned)dm.num_pages) unit(kc, vc, u + NWV);
     }
-    if (i < n_mine && (unsigned)pg_a < (unsigned)dm.num_pages) unit(ka, va, u);
+    if (i + 1 < n_mine) {
+      pg_c = next_page(i + 1);
+      issue(kc, vc, pg_c, (u + NWV) & 1);
+      if ((unsigned)pg_a < (unsigned)dm.num_pages) unit(ka, va, u);
+      if ((unsigned)pg_c < (unsigned)dm.num_pages) unit(kc, vc, u + NWV);
+    } else if (i < n_mine && (unsigned)pg_a < (unsigned)dm.num_pages) {
+      unit(ka, va, u);
+    }
   }
   // park the partial results: accumulator register i of tile mt in lane (row = col, j) is feature mt*16 + 4j + i
   __builtin_amdgcn_wave_barrier();
