@@ -300,7 +300,9 @@ __device__ __forceinline__ void paged_redo_row(const PagedDims& dm, const PagedO
 // ---- few rows ----------------------------------------------------------------------------------
 // 16 NR rows a workgroup; units of 32 tokens (half a page) go to its wavefronts in turn, the next unit's keys and values
 // under way while one is worked on; the wavefronts' results meet in LDS.  K rows are read straight into A operands (a lane 16
-// bytes of its token's row), V goes through the wavefront's own LDS area and is read by the transposing load.
+// bytes of its token's row), V goes through the wavefront's own LDS area and is read by the transposing load.  Bound by HBM:
+// a token of 16 sequences of 16K to 32K, 8 KV heads of 128, 237 us (1.54 GB: 6.5 TB/s, a plain read reaches 6.9), and with a
+// window of 512 by the latencies around it: 32 such sequences 14.3 us (74 MB), one of 2 KV heads of 64 5.6 us.
 template <int D, int NR, int NWV, bool TREE, bool PAST>
 __global__ void __launch_bounds__(NWV * 64) __attribute__((amdgpu_waves_per_eu(NR == 2 && D == 128 ? 1 : 2)))
 paged_attn_rows(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, const bf16_t* __restrict__ v, PagedDims dm,
@@ -568,6 +570,9 @@ paged_attn_rows(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, cons
 // wavefront overlap, those of two that run in step hardly do).  The exponentials' reference point follows a row's maximum
 // only when a score is more than 2^6 above it: the others need no reduction over lanes and no rescaling, and probabilities
 // of up to 2^6 enter sum and output alike.
+// Bound by latencies where a window has ten pages (17.4 us for trees of 63 tokens for 8 sequences, 8 KV heads of 128: 7.6 in
+// the steps), else by the vector and matrix units together: 1.6 us a page of 256 rows, 0.85 of it matrix products; trees of 64
+// tokens for 4 sequences of 8K to 16K, 4 KV heads of 128, everything seen: 72 us with the join (51 GFLOP).
 // The buffers come first: their places are then plain offsets, and a buffer's number is two bits of them.
 template <int D, int NW, int KW, bool TREE>
 static constexpr size_t paged_tiles_smem() {
@@ -990,7 +995,7 @@ paged_attn_tiles(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, con
 
 // ---- shares of a range added up ------------------------------------------------------------------
 // A wavefront a row: lane i weighs share i (there are up to 64), then groups of D / 4 lanes take every GR-th share, four loads
-// under way, and add up across the groups.
+// under way, and add up across the groups.  Bound by HBM or the launch: 32768 rows of 8 shares (34 MB) in 7.5 to 10 us.
 template <int D>
 __global__ void __launch_bounds__(256) paged_attn_join(PagedDims dm, PagedOut out) {
   constexpr int LPR = D / 4, GR = 64 / LPR;  // lanes per row of features, groups

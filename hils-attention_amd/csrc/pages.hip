@@ -98,7 +98,8 @@ extern "C" int hils_copy_pages(void** pools, const size_t* page_bytes, const voi
 // Token path[b][i] of the drafts behind `base` committed tokens becomes the sequence's token base + i: its key and value
 // move from slot base + path[b][i] to slot base + i.  Only the longest start of a path that grows strictly counts (a
 // negative entry ends it), so path[i] >= i and no move overwrites what a later one reads: a thread owns 16 bytes of
-// every token and moves eight tokens at a time, all eight read before the first is written.
+// every token and moves eight tokens at a time, all eight read before the first is written.  Bound by its latencies (path and
+// table, values, stores): 3 to 5 us.
 #define ACC_MAX 256
 
 __global__ void __launch_bounds__(256)
