@@ -97,17 +97,20 @@ __device__ __forceinline__ int paged_ragged(const PagedDims& dm, int lane, int l
 }
 
 // What a workgroup works on: share `share` of `of` of a sequence's pages.  The row blocks of a (share, KV head) read the same
-// pages: neighbours on one XCD (the hardware hands consecutive workgroups to the eight XCDs in turn).  `slot` numbers the
+// pages: neighbours on one XCD (the hardware hands consecutive workgroups to the eight XCDs in turn); so do the VS workgroups
+// that have a part of the values' features each.  `slot` numbers the
 // shares of all sequences (it is the sequence where none is split).  False for what is left over at the end.
 struct PagedUnit {
-  int blk, hk, slot, b, share, of, len;
+  int blk, vs, hk, slot, b, share, of, len;
 };
+template <int VS>
 __device__ __forceinline__ bool paged_unit(const PagedDims& dm, int lane, PagedUnit& u) {
-  const int total = dm.n_blk * dm.n_split * dm.H * dm.B, per_xcd = (total + 7) / 8;
+  const int total = dm.n_blk * VS * dm.n_split * dm.H * dm.B, per_xcd = (total + 7) / 8;
   const int id = (int)(blockIdx.x % 8) * per_xcd + (int)(blockIdx.x / 8);
   if (id >= total) return false;
-  const int rest = id / dm.n_blk;
-  u.blk = id - rest * dm.n_blk;
+  const int part = id / VS, rest = part / dm.n_blk;
+  u.vs = id - part * VS;
+  u.blk = part - rest * dm.n_blk;
   u.slot = rest / dm.H;
   u.hk = rest - u.slot * dm.H;
   if (dm.ragged) {
@@ -232,13 +235,16 @@ __device__ __forceinline__ void paged_store4(const PagedDims& dm, const PagedOut
 }
 
 // One row over the pages p0 .. p1 - 1, by one wavefront, looking at no token that the row does not see.
-template <int D>
+template <int D, int VS>
 __device__ __forceinline__ void paged_redo_row(const PagedDims& dm, const PagedOut& out, const bf16_t* qr, const bf16_t* k,
                                             const bf16_t* v, const int32_t* table, int hk, int base, int p0, int p1, int t,
-                                            int left, const unsigned* mask_row, long row, int lane) {
-  float m = HILS_NEG_INF, l = 0.f, x[D / 64];
+                                            int left, const unsigned* mask_row, long row, int vs, int lane) {
+  constexpr int DV = D / VS, NF = DV > 64 ? DV / 64 : 1;
+  const bool mine = DV >= 64 || lane < DV;  // lanes that have features of the DV from f0 on
+  const int f0 = vs * DV + (mine ? lane : 0);
+  float m = HILS_NEG_INF, l = 0.f, x[NF];
 #pragma unroll
-  for (int f = 0; f < D / 64; ++f) x[f] = 0.f;
+  for (int f = 0; f < NF; ++f) x[f] = 0.f;
   for (int p = p0; p < p1; ++p) {
     const int page = table[p];
     if ((unsigned)page >= (unsigned)dm.num_pages) continue;
@@ -270,21 +276,22 @@ __device__ __forceinline__ void paged_redo_row(const PagedDims& dm, const PagedO
     m = m_new;
     l = l * corr + wave_sum(e);
 #pragma unroll
-    for (int f = 0; f < D / 64; ++f) x[f] *= corr;
+    for (int f = 0; f < NF; ++f) x[f] *= corr;
     uint64_t who = __ballot(see);
     while (who) {
       const int i = __builtin_ctzll(who);
       who &= who - 1;
       const float pe = __shfl(e, i, 64);
 #pragma unroll
-      for (int f = 0; f < D / 64; ++f) x[f] = fmaf(pe, bf2f(v[at + (long)i * D + f * 64 + lane]), x[f]);
+      for (int f = 0; f < NF; ++f) x[f] = fmaf(pe, bf2f(v[at + (long)i * D + f * 64 + f0]), x[f]);
     }
   }
   if (dm.n_split > 1) {
     float* part = out.part + row * D;
 #pragma unroll
-    for (int f = 0; f < D / 64; ++f) part[f * 64 + lane] = x[f];
-    if (lane == 0) {
+    for (int f = 0; f < NF; ++f)
+      if (mine) part[f * 64 + f0] = x[f];
+    if (lane == 0 && vs == 0) {
       float* ml = out.part + out.n_rows * dm.n_split * D + row * 2;
       ml[0] = m;
       ml[1] = l;
@@ -293,8 +300,9 @@ __device__ __forceinline__ void paged_redo_row(const PagedDims& dm, const PagedO
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-  for (int f = 0; f < D / 64; ++f) out.o[row * D + f * 64 + lane] = f2bf(x[f] * inv);
-  if (lane == 0) out.lse[row] = l == 0.f ? HILS_NEG_INF : (m * dm.c2 + __builtin_amdgcn_logf(l)) * HILS_LN2;
+  for (int f = 0; f < NF; ++f)
+    if (mine) out.o[row * D + f * 64 + f0] = f2bf(x[f] * inv);
+  if (lane == 0 && vs == 0) out.lse[row] = l == 0.f ? HILS_NEG_INF : (m * dm.c2 + __builtin_amdgcn_logf(l)) * HILS_LN2;
 }
 
 // ---- few rows ----------------------------------------------------------------------------------
@@ -302,14 +310,16 @@ __device__ __forceinline__ void paged_redo_row(const PagedDims& dm, const PagedO
 // under way while one is worked on; the wavefronts' results meet in LDS.  K rows are read straight into A operands (a lane 16
 // bytes of its token's row), V goes through the wavefront's own LDS area and is read by the transposing load.  Bound by HBM:
 // a token of 16 sequences of 16K to 32K, 8 KV heads of 128, 237 us (1.54 GB: 6.5 TB/s, a plain read reaches 6.9), and with a
-// window of 512 by the latencies around it: 32 such sequences 14.3 us (74 MB), one of 2 KV heads of 64 5.6 us.
-template <int D, int NR, int NWV, bool TREE, bool PAST>
+// window of 512 by the latencies around it: 32 such sequences 14.3 us (74 MB), one of 2 KV heads of 64 5.6 us.  Where there
+// are few of them a workgroup is bound by what its compute unit takes in (some 65 GB/s): then VS of them have a part of the
+// values' features each and all keys (1 to 8 sequences, 8 KV heads of 128, window 512: 8.7 us alone, 7.8 by two, 7.5 by four).
+template <int D, int NR, int NWV, bool TREE, bool PAST, int VS>
 __global__ void __launch_bounds__(NWV * 64) __attribute__((amdgpu_waves_per_eu(NR == 2 && D == 128 ? 1 : 2)))
 paged_attn_rows(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, const bf16_t* __restrict__ v, PagedDims dm,
                 PagedOut out) {
-  constexpr int KS = D / 32, MT = D / 16, ROWS = 16 * NR;
-  constexpr int VL = D / 8, TPI = 64 / VL, VI = 32 / TPI;  // lanes per V row, rows per load, loads per unit
-  constexpr int VP = 2 * D + 16, OP = D + 4;
+  constexpr int DV = D / VS, KS = D / 32, MT = DV / 16, ROWS = 16 * NR;
+  constexpr int VL = DV / 8, TPI = 64 / VL, VI = 32 / TPI;  // lanes per V row, rows per load, loads per unit
+  constexpr int VP = 2 * DV + 16, OP = DV + 4;
   constexpr int AREA = 32 * VP > ROWS * OP * 4 ? 32 * VP : ROWS * OP * 4;
   __shared__ __align__(16) unsigned char area_s[NWV * AREA];
   __shared__ float m_s[NWV][ROWS], l_s[NWV][ROWS];
@@ -319,7 +329,7 @@ paged_attn_rows(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, cons
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, j = lane >> 4;
   PagedUnit at;
-  if (!paged_unit(dm, lane, at)) return;
+  if (!paged_unit<VS>(dm, lane, at)) return;
   const int blk = at.blk, hk = at.hk, b = at.b;
   const int n_rows = dm.T * dm.G, r0 = blk * ROWS;
   const int r1 = r0 + ROWS < n_rows ? r0 + ROWS : n_rows;
@@ -350,7 +360,7 @@ paged_attn_rows(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, cons
     for (int ks = 0; ks < KS; ++ks) qb[rt][ks] = *(const bf16x8_t*)(qp + ks * 32);
   }
   const bf16_t* kb = k + (long)hk * PA_PAGE * D + col * D + j * 8;
-  const bf16_t* vb = v + (long)hk * PA_PAGE * D + lane * 8;
+  const bf16_t* vb = v + (long)hk * PA_PAGE * D + lane / VL * D + lane % VL * 8 + at.vs * DV;
   const long page_el = (long)dm.H * PA_PAGE * D;
   auto issue = [&](pa_u4 (&kd)[2][KS], pa_u4 (&vd)[VI], int page, int half) __attribute__((always_inline)) {
     const long at = (unsigned)page < (unsigned)dm.num_pages ? page * page_el : 0;  // (not mapped: not worked on)
@@ -524,8 +534,8 @@ paged_attn_rows(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, cons
     }
   }
   __syncthreads();
-  for (int p = tid; p < ROWS * (D / 4); p += NWV * 64) {
-    const int rr = p / (D / 4), d4 = p % (D / 4), r = r0 + rr;
+  for (int p = tid; p < ROWS * (DV / 4); p += NWV * 64) {
+    const int rr = p / (DV / 4), d4 = p % (DV / 4), r = r0 + rr;
     if (r >= r1) continue;
     float M = HILS_NEG_INF;
 #pragma unroll
@@ -543,7 +553,7 @@ paged_attn_rows(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, cons
     }
     const int t = hils_udiv(r, dm.G, dm.g_magic), g = r - t * dm.G;
     const long row = ((long)at.slot * dm.T + t) * dm.HQ + hk * dm.G + g;
-    paged_store4<D>(dm, out, row, d4, x, M, L);
+    paged_store4<D>(dm, out, row, at.vs * (DV / 4) + d4, x, M, L);
     const float all = (x[0] + x[1]) + (x[2] + x[3]);  // (no finite number if one of them is none)
     if (!(fabsf(all) < INFINITY)) atomicOr(&odd_s, 1u << rr);
   }
@@ -554,8 +564,8 @@ paged_attn_rows(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, cons
       const int r = r0 + rr, t = hils_udiv(r, dm.G, dm.g_magic), g = r - t * dm.G;
       const long row = ((long)at.slot * dm.T + t) * dm.HQ + hk * dm.G + g;
       int left = TREE ? left_s[t - t0] : paged_left(sp.base + t, dm);
-      paged_redo_row<D>(dm, out, q + b * dm.q_sb + t * dm.q_st + (hk * dm.G + g) * dm.q_sh, k, v, table, hk, sp.base, sp.p0,
-                        sp.p1, t, left, TREE ? mask_s + (t - t0) * PA_WORDS : nullptr, row, lane);
+      paged_redo_row<D, VS>(dm, out, q + b * dm.q_sb + t * dm.q_st + (hk * dm.G + g) * dm.q_sh, k, v, table, hk, sp.base, sp.p0,
+                        sp.p1, t, left, TREE ? mask_s + (t - t0) * PA_WORDS : nullptr, row, at.vs, lane);
     }
   }
 }
@@ -596,7 +606,7 @@ paged_attn_tiles(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, con
   const int col = lane & 31, h = lane >> 5;
   const int rg = wave % RW, kg = wave / RW;  // rows and half of every page (KW == 2) that are this wavefront's
   PagedUnit at;
-  if (!paged_unit(dm, lane, at)) return;
+  if (!paged_unit<1>(dm, lane, at)) return;
   const int blk = at.blk, hk = at.hk, b = at.b;
   const int n_rows = dm.T * dm.G, r0 = blk * ROWS;
   const int r1 = r0 + ROWS < n_rows ? r0 + ROWS : n_rows;
@@ -986,9 +996,9 @@ paged_attn_tiles(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, con
       odd &= odd - 1;
       const int rr = r0 + rg * 32 + i, tr = hils_udiv(rr, dm.G, dm.g_magic), gr = rr - tr * dm.G;
       const int left = TREE ? left_s[tr - t0] : paged_left(sp.base + tr, dm);
-      paged_redo_row<D>(dm, out, q + b * dm.q_sb + tr * dm.q_st + (hk * dm.G + gr) * dm.q_sh, k, v, table, hk, sp.base, sp.p0,
+      paged_redo_row<D, 1>(dm, out, q + b * dm.q_sb + tr * dm.q_st + (hk * dm.G + gr) * dm.q_sh, k, v, table, hk, sp.base, sp.p0,
                         sp.p1, tr, left, TREE ? mask_s + (tr - t0) * PA_WORDS : nullptr,
-                        ((long)at.slot * dm.T + tr) * dm.HQ + hk * dm.G + gr, lane);
+                        ((long)at.slot * dm.T + tr) * dm.HQ + hk * dm.G + gr, 0, lane);
     }
   }
 }
@@ -1054,6 +1064,7 @@ __global__ void __launch_bounds__(256) paged_attn_join(PagedDims dm, PagedOut ou
 struct PagedPlan {
   bool past;           // values are read past the caches
   int rows, nw, kw;    // rows a workgroup; wavefronts of the tile kernel and those that share a row (0: the row kernel)
+  int vs;              // workgroups of a row block that have a part of the values' features each
   int n_blk, n_split;
 };
 
@@ -1061,20 +1072,23 @@ struct PagedPlan {
 // What the variants cost, in microseconds, from sweeps of every variant and share count over 1 to 32 sequences, 1 to 128 new
 // tokens, windows of 512 tokens and contexts of 512 to 32768: a launch is about
 //   fixed + rounds * (start + page * pages of a share)
-// or, where that is longer, the bytes read once at 6.8 TB/s or those that all workgroups read at 21 TB/s; a round is one
+// or, where that is longer, the bytes read once at 7 TB/s or those that all workgroups read at 19.5 TB/s; a round is one
 // workgroup on every compute unit, and where a second one fits beside it (heads of 64) the two take (1 + beside) rounds.  More
-// than one share adds the join, its results written and read at 3.2 TB/s.  The choice that this predicts to be shortest was
-// within 2 % of the best measured one on average and within 17 % in the worst of 159 calls; fixed
+// than one share adds the join, its results written and read at 3.1 TB/s.  The choice that this predicts to be shortest was
+// within 2 % of the best measured one on average and within 17 % in the worst of 187 calls; fixed
 // thresholds on rows and pages were 15 % off on average and lost up to 1.7 times (1 token, 8 KV heads of 128, 4096 tokens: 8
 // shares 12.9 us, 32 shares 8.5; 16 tokens, 2 KV heads of 64, window 512: 32 rows a workgroup 10.1, 16 rows 7.5).
 struct PagedCost {
-  int rows, nw, kw;
+  int rows, vs, nw, kw;
   float fixed, start, page, beside;
 };
-static const PagedCost kPagedCost128[] = {{16, 0, 0, 1.8f, 4.0f, 0.56f, 1.f}, {32, 0, 0, 3.5f, 4.0f, 0.73f, 1.f}, {64, 4, 2, 4.8f, 2.7f, 0.76f, 1.f},
-                                          {128, 8, 2, 6.0f, 2.8f, 0.95f, 1.f}, {256, 8, 1, 6.9f, 0.3f, 1.60f, 1.f}};
-static const PagedCost kPagedCost64[] = {{16, 0, 0, 2.8f, 1.9f, 0.28f, 0.94f}, {32, 0, 0, 3.6f, 2.1f, 0.48f, 0.42f}, {64, 4, 2, 4.1f, 2.7f, 0.57f, 0.38f},
-                                         {128, 4, 1, 6.9f, 0.f, 0.89f, 0.49f}};
+static const PagedCost kPagedCost128[] = {{16, 1, 0, 0, 1.1f, 3.9f, 0.53f, 1.f}, {16, 2, 0, 0, 1.0f, 3.5f, 0.44f, 1.f},
+                                          {16, 4, 0, 0, 1.0f, 3.1f, 0.42f, 1.f}, {32, 1, 0, 0, 3.9f, 3.8f, 0.74f, 1.f},
+                                          {64, 1, 4, 2, 4.9f, 2.4f, 0.76f, 1.f}, {128, 1, 8, 2, 6.4f, 2.1f, 0.95f, 1.f},
+                                          {256, 1, 8, 1, 6.9f, 0.f, 1.59f, 1.f}};
+static const PagedCost kPagedCost64[] = {{16, 1, 0, 0, 2.3f, 2.2f, 0.26f, 0.81f}, {16, 2, 0, 0, 2.4f, 1.9f, 0.21f, 0.81f},
+                                         {32, 1, 0, 0, 3.7f, 1.9f, 0.47f, 0.49f}, {64, 1, 4, 2, 4.3f, 2.1f, 0.56f, 0.46f},
+                                         {128, 1, 4, 1, 6.3f, 0.f, 0.88f, 0.53f}};
 
 static PagedPlan paged_choose(int B, int T, int HQ, int H, int D, int window, int max_pages) {
   PagedPlan best = {};
@@ -1084,31 +1098,32 @@ static PagedPlan paged_choose(int B, int T, int HQ, int H, int D, int window, in
     const long pages = ((long)window + tokens + 2 * PA_PAGE - 3) / PA_PAGE;
     return pages < max_pages ? pages : max_pages;
   };
-  const float read = (float)B * H * pages_of(T) * PA_PAGE * D * 4 / 6.8e6f;
+  const float read = (float)B * H * pages_of(T) * PA_PAGE * D * 4 / 7e6f;
   // Sequences of a batch differ in length where the window does not make their ranges alike, and the last workgroups run alone:
   // smaller ones are better by about a twentieth of one's time (16 sequences of 16K to 32K, 8 KV heads of 128: 2 shares 255 us,
   // 4 shares 237; all of 8K: 81 and 85).
   const bool uneven = B > 1 && pages_of(T) == max_pages;
   float least = 0.f;
   const PagedCost* cost = D == 128 ? kPagedCost128 : kPagedCost64;
-  for (int i = 0; i < (D == 128 ? 5 : 4); ++i) {
+  for (int i = 0; i < (D == 128 ? 7 : 5); ++i) {
     const PagedCost& c = cost[i];
     const int per = c.rows;
-    if (i && rows <= per / 2) break;  // (the variants before hold every row with fewer of them empty)
+    if (per > 16 && rows <= per / 2) break;  // (the variants before hold every row with fewer of them empty)
     const long n_blk = (rows + per - 1) / per, tokens = per / G + 1 > PA_MAX_TREE ? per / G + 1 : PA_MAX_TREE;
     const long pages = pages_of(T < tokens ? T : tokens);
     for (int n_split = 1; n_split <= 64 && (n_split == 1 || 2 * n_split <= pages); n_split += n_split < 4 ? 1 : n_split / 4) {
-      const long n = (n_blk * n_split * H * B + cus - 1) / cus;
+      const long wgs = n_blk * c.vs * n_split * H * B, n = (wgs + cus - 1) / cus;
       const float rounds = c.beside < 1.f ? (n / 2) * (1.f + c.beside) + n % 2 : (float)n;
       const float one = c.start + c.page * ((pages + n_split - 1) / n_split), work = rounds * one;
-      const float near = (float)n_blk * n_split * H * B * ((pages + n_split - 1) / n_split) * PA_PAGE * D * 4 / 21e6f;
+      const float near = (float)wgs * ((pages + n_split - 1) / n_split) * PA_PAGE * D * 2 * (1.f + 1.f / c.vs) / 19.5e6f;
       // (the fourth powers: a sweep near two bounds takes longer than either)
       const auto fourth = [](float x) { return x * x * x * x; };
       float t = c.fixed + (uneven ? 0.05f * one : 0.f) + sqrtf(sqrtf(fourth(work) + fourth(read) + fourth(near)));
-      if (n_split > 1) t += 2.9f + (float)B * rows * H * n_split * (D + 2) * 8 / 3.2e6f;
+      if (n_split > 1) t += 3.5f + (float)B * rows * H * n_split * (D + 2) * 8 / 3.1e6f;
       if (best.n_blk && t >= least) continue;
       least = t;
       best.rows = c.rows;
+      best.vs = c.vs;
       best.nw = c.nw;
       best.kw = c.kw;
       best.n_blk = (int)n_blk;
@@ -1119,7 +1134,7 @@ static PagedPlan paged_choose(int B, int T, int HQ, int H, int D, int window, in
   // 16K to 32K, 8 KV heads of 128 (1.54 GB): 277 -> 255 us; where they fit, and are there from the call before, that would lose
   // (32768 tokens, 8 heads of 128: 28 -> 33 us).  Keys are read 64 bytes of a row at a time, half a cache line, and lose by it
   // at any size.
-  best.past = best.n_blk == 1 && (double)B * H * pages_of(T) * PA_PAGE * D * 4 > HILS_LAST_CACHE;
+  best.past = best.n_blk == 1 && best.vs == 1 && (double)B * H * pages_of(T) * PA_PAGE * D * 4 > HILS_LAST_CACHE;
   return best;
 }
 
@@ -1147,7 +1162,7 @@ extern "C" size_t hils_paged_attn_workspace(int B, int T, int HQ, int H, int D, 
 template <int D, bool TREE>
 static int paged_launch(const PagedPlan& pl, const bf16_t* q, const bf16_t* k, const bf16_t* v, const PagedDims& dm,
                         const PagedOut& out, hipStream_t st) {
-  const dim3 grid((unsigned)(((long)dm.n_blk * dm.n_split * dm.H * dm.B + 7) / 8 * 8));
+  const dim3 grid((unsigned)(((long)dm.n_blk * pl.vs * dm.n_split * dm.H * dm.B + 7) / 8 * 8));
 #define PA_TILES(NW_, KW_)                                                                           \
   do {                                                                                               \
     static HilsLdsReserve reserved;                                                                  \
@@ -1156,9 +1171,12 @@ static int paged_launch(const PagedPlan& pl, const bf16_t* q, const bf16_t* k, c
     if (int rc = hils_reserve_lds(&reserved, (const void*)kern, smem, "hils_paged_attn")) return rc; \
     hipLaunchKernelGGL(kern, grid, dim3(NW_ * 64), smem, st, q, k, v, dm, out);                      \
   } while (0)
-  if (pl.rows == 16 && pl.past) hipLaunchKernelGGL((paged_attn_rows<D, 1, 8, TREE, true>), grid, dim3(512), 0, st, q, k, v, dm, out);
-  else if (pl.rows == 16) hipLaunchKernelGGL((paged_attn_rows<D, 1, 8, TREE, false>), grid, dim3(512), 0, st, q, k, v, dm, out);
-  else if (pl.rows == 32) hipLaunchKernelGGL((paged_attn_rows<D, 2, 4, TREE, false>), grid, dim3(256), 0, st, q, k, v, dm, out);
+  constexpr int VS4 = D == 128 ? 4 : 2;  // (heads of 64 gain nothing by four)
+  if (pl.vs == 4) hipLaunchKernelGGL((paged_attn_rows<D, 1, 8, TREE, false, VS4>), grid, dim3(512), 0, st, q, k, v, dm, out);
+  else if (pl.vs == 2) hipLaunchKernelGGL((paged_attn_rows<D, 1, 8, TREE, false, 2>), grid, dim3(512), 0, st, q, k, v, dm, out);
+  else if (pl.rows == 16 && pl.past) hipLaunchKernelGGL((paged_attn_rows<D, 1, 8, TREE, true, 1>), grid, dim3(512), 0, st, q, k, v, dm, out);
+  else if (pl.rows == 16) hipLaunchKernelGGL((paged_attn_rows<D, 1, 8, TREE, false, 1>), grid, dim3(512), 0, st, q, k, v, dm, out);
+  else if (pl.rows == 32) hipLaunchKernelGGL((paged_attn_rows<D, 2, 4, TREE, false, 1>), grid, dim3(256), 0, st, q, k, v, dm, out);
   else if (pl.rows == 64) PA_TILES(4, 2);
   else if constexpr (D == 64) PA_TILES(4, 1);
   else if (pl.rows == 128) PA_TILES(8, 2);
@@ -1191,7 +1209,7 @@ extern "C" int hils_paged_attn(const void* q, const void* k_pages, const void* v
                "hils_paged_attn: q's strides and address must be multiples of 16 bytes");
   const PagedPlan pl = paged_plan(B, T, HQ, H, D, window, max_pages);
   const long rows = (long)B * T * HQ;
-  HILS_REQUIRE((long)pl.n_blk * pl.n_split * H * B < (1l << 31) - 8, "hils_paged_attn: sizes too large for the grid");
+  HILS_REQUIRE((long)pl.n_blk * pl.vs * pl.n_split * H * B < (1l << 31) - 8, "hils_paged_attn: sizes too large for the grid");
   const size_t need = paged_ws(pl, rows, D);
   HILS_REQUIRE(need == 0 || (workspace && workspace_bytes >= need),
                "hils_paged_attn: workspace too short: %zu bytes, %zu needed", workspace_bytes, need);
