@@ -46,7 +46,8 @@ def paged_flex_attn(q, k_pages, v_pages, page_table, seq_len, window_size, paren
     int32 (T,) or (B,T): token t follows the new token parents[t] < t, or the last committed one (-1); it sits at position
     seq_len - T + depth and sees the committed tokens of its window, itself and its ancestors.  Tokens with any other parent,
     and those that follow them, see nothing (padding).  Without ``parents`` the tokens are a chain.  T <= 256 for a tree.
-    Returns o (B,T,H_q,D) bf16 and lse (B,T,H_q) fp32, natural log; rows that see nothing: 0 and -inf."""
+    Returns o (B,T,H_q,D) bf16 and lse (B,T,H_q) fp32, natural log; rows that see nothing: 0 and -inf.  The same call gives
+    the same bits; a sequence's last bits may depend on how many others, and how long ones, are in the batch."""
     args = (q, k_pages, v_pages, page_table, seq_len, int(window_size), parents, bool(mask_lmk), bool(expand_to_chunk), sm_scale)
     if q.requires_grad or k_pages.requires_grad or v_pages.requires_grad:
         return _inference("paged_flex_attn", lambda: _cabi.host().paged_flex_attn(*args), q, k_pages, v_pages)

@@ -155,3 +155,58 @@ def test_captured_and_replayed(pkg, dev):
                 assert torch.equal(w, x) and torch.equal(w, y)
                 x.zero_()
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("HQ,H,D", [(8, 2, 128), (16, 2, 64), (4, 1, 128)])
+@pytest.mark.parametrize("T,tree", [(1, False), (6, True), (70, True)])
+def test_stale_numbers_in_some_features(pkg, dev, HQ, H, D, T, tree):
+    """A NaN in one feature of a hidden value: what computes the other features of the row does not see it."""
+    note(f"stale numbers in some features, T{T} heads {HQ}/{H} x {D}")
+    for feature, ctx, window in ((0, 700, 200), (D - 1, 700, 1 << 20), (D // 2, 5000, 1 << 20)):
+        q, k, v, table, lengths, parents = _inputs(dev, D, HQ, H, 2, T, ctx, tree, seed=T + feature)
+        lengths[1] = ctx - 70
+        want = ref.attend_dense(q, k, v, table, lengths, window, parents)
+        for b in range(2):
+            see = ref.visible(T, int(lengths[b]), window, None if parents is None else parents[b].tolist(), True, True, table.shape[1] * 64)
+            at = (~see.any(0)).nonzero().flatten().to(dev)
+            v[table[b, at // 64].long(), :, at % 64, feature] = float("nan")
+        got = _call(pkg, q, k, v, table, lengths, window, parents)
+        ref.check_attention(got, want)
+        again = _call(pkg, q, k, v, table, lengths, window, parents)
+        assert all(torch.equal(x, y) for x, y in zip(got, again))
+
+
+def test_a_captured_step_over_growing_sequences(pkg, dev):
+    """Append and attend of a ragged batch in a graph whose lengths grow on the GPU, replay by replay, against eager calls."""
+    note("a captured step, lengths growing")
+    for HQ, H, D, lens, window in ((16, 2, 64, [40, 700, 63, 3000], 1 << 20), (8, 2, 128, [5, 9000, 127, 6000], 1 << 20),
+                                   (32, 8, 128, [511, 512, 64, 1], 100)):
+        B, n = len(lens), 145
+        gen = torch.Generator().manual_seed(D)
+        k, v, table = ref.cache(gen, B, n, H, D, dev)
+        inv, scale = pkg.rotary_frequencies(D, device=dev)
+        new = [torch.randn(B, 1, h, D, generator=gen).bfloat16().to(dev) for h in (HQ, H, H)]
+
+        def step(kp, vp, lengths):
+            lengths.add_(1)
+            q = pkg.paged_append(new[1], new[2], kp, vp, table, lengths, q=new[0], inv_freq=inv, scale=scale)
+            return pkg.paged_flex_attn(q, kp, vp, table, lengths, window)
+
+        mine, lengths = (k.clone(), v.clone()), torch.tensor(lens, dtype=torch.int32, device=dev)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step(k.clone(), v.clone(), lengths.clone())
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=side):
+                out = step(*mine, lengths)
+        torch.cuda.synchronize()
+        at = torch.tensor(lens, dtype=torch.int32, device=dev)
+        assert torch.equal(at, lengths)  # (captured, not run)
+        for _ in range(70):  # (past a page's end for every sequence)
+            g.replay()
+            want = step(k, v, at)
+            assert all(torch.equal(x, y) for x, y in zip(out, want))
+        torch.cuda.synchronize()
+        assert torch.equal(at, lengths) and torch.equal(mine[0], k) and torch.equal(mine[1], v)
+        ref.check_attention(want, ref.attend_dense(pkg.rotary_embedding(new[0], None, (at - 1).view(B, 1), inv, scale=scale)[0], k, v, table, at, window))
