@@ -126,8 +126,9 @@ rotary_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, const 
   if (APPEND && tid < n) {
     int b, t;
     token(tid, b, t);
-    const int slot = (dm.lengths ? dm.lengths[b] : dm.seq_len) - dm.T + t, c = slot >> 6;
-    const int page = slot >= 0 && c < dm.max_pages ? dm.table[(long)b * dm.max_pages + c] : -1;
+    const int len = dm.lengths ? dm.lengths[b] : dm.seq_len, slot = len - dm.T + t, c = slot >> 6;
+    // (a sequence shorter than T takes no part: the tokens that it has stay as they are)
+    const int page = len >= dm.T && c < dm.max_pages ? dm.table[(long)b * dm.max_pages + c] : -1;
     slot_s[tid] = (unsigned)page < (unsigned)dm.num_pages ? (long)page * dm.H * 64 + (slot & 63) : -1;
   }
   for (int i = tid; i < n * half; i += 256) {

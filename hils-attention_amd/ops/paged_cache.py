@@ -2,7 +2,8 @@
 
 The layouts are those of ``HiLSPagedLayer`` and ``paged_hils_attend``: k_pages, v_pages (num_pages, H, 64, D) bf16,
 page_table (B, max_pages) int32 (entries outside the pool: not mapped).  Lengths are an int for all sequences or an int32
-tensor (B,) on the GPU.  Everything runs on the current stream and synchronises nothing; inference only.
+tensor (B,) on the GPU; a sequence shorter than the T tokens of a call takes no part in it.  Everything runs on the current
+stream and synchronises nothing; inference only.
 """
 import torch
 
@@ -29,7 +30,7 @@ def _inference(name, call, *inputs):
 def paged_append(k, v, k_pages, v_pages, page_table, seq_len, q=None, inv_freq=None, positions=None, interleaved=False,
                  scale=1.0):
     """Write keys and values (B,T,H,D) of the last T of ``seq_len`` tokens into their pages, in one launch; tokens whose
-    page is not mapped are left out.  With ``inv_freq`` the keys, and q (B,T,H_q,D) if given, are rotated on the way as by
+    page is not mapped, and sequences shorter than T, are left out.  With ``inv_freq`` the keys, and q (B,T,H_q,D) if given, are rotated on the way as by
     ``rotary_embedding``, at ``positions`` (B,T) or, without them, at the tokens' slots.  Returns the rotated q or None."""
     args = (k, v, k_pages, v_pages, page_table, seq_len, q, inv_freq, positions, bool(interleaved), float(scale))
     if k.requires_grad or v.requires_grad or (q is not None and q.requires_grad):

@@ -472,7 +472,7 @@ int hils_rotary(const void* q, const void* k, void* q_out, void* k_out, const vo
 /* Layouts of the paged cache as above: k_pages, v_pages (num_pages,H,64,D) bf16, page_table (B,max_pages) int32, chunk c of a
  * sequence -> page (negative or >= num_pages: not mapped; nothing is written there and nobody sees what would lie there).
  * lengths (B) int32: tokens of every sequence, the T new ones included; NULL: seq_len for all.  A sequence shorter than T
- * takes no part.
+ * takes no part: none of its pages are written, its rows of the attention are 0 (lse -inf), its rows of q_out mean nothing.
  *
  * hils_paged_append: keys and values (B,T,H,D) of the last T tokens (slots length - T ..) into their pages, and q (B,T,HQ,D)
  * into q_out (HQ = 0: none).  With rotary_dim > 0 q and k are rotated as by hils_rotary, at positions (B,T), NULL: the

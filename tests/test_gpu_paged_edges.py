@@ -1,0 +1,35 @@
+"""Calls at the edges of what the operators on a paged cache take: sequences too short for the call, layouts of single rows,
+numbers left behind by whoever had the pages before."""
+import pytest
+import torch
+
+import paged_ref as ref
+from util import note
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("heads", [(16, 2, 64), (32, 8, 128)])
+@pytest.mark.parametrize("T", [2, 8, 70])
+@pytest.mark.parametrize("turned", [False, True])
+def test_append_leaves_short_sequences_alone(pkg, dev, heads, T, turned):
+    """A sequence with fewer tokens than the call has new ones keeps every byte of its pages, all of them mapped."""
+    note(f"append of {T} tokens beside shorter sequences, heads {heads}, rotated {turned}")
+    HQ, H, D = heads
+    lengths = [1, T - 1, T, 0, -1, T // 2, T + 1, 150]
+    gen = torch.Generator().manual_seed(T)
+    kp, vp, table = ref.cache(gen, len(lengths), 3, H, D, dev)
+    k, v = (torch.randn(len(lengths), T, H, D, generator=gen).bfloat16().to(dev) for _ in range(2))
+    inv, _ = pkg.rotary_frequencies(D, device=dev)
+    ln = torch.tensor(lengths, dtype=torch.int32, device=dev)
+    want_k, want_v = kp.clone(), vp.clone()
+    # (the keys as the operator itself turns them: what is tested is where they go)
+    at = ln.view(-1, 1) - T + torch.arange(T, device=dev)
+    turned_k = pkg.rotary_embedding(k, None, at, inv)[0] if turned else k
+    for b, n in enumerate(lengths):
+        for t in range(T if n >= T else 0):
+            slot = n - T + t
+            page = table[b, slot // 64].long()
+            want_k[page, :, slot % 64], want_v[page, :, slot % 64] = turned_k[b, t], v[b, t]
+    pkg.paged_append(k, v, kp, vp, table, ln, inv_freq=inv if turned else None)
+    assert torch.equal(kp, want_k) and torch.equal(vp, want_v)
