@@ -1207,6 +1207,9 @@ extern "C" int hils_paged_attn(const void* q, const void* k_pages, const void* v
   HILS_REQUIRE(B <= 65535 && H <= 65535 && (long)T * (HQ / H) * (HQ / H) < (1l << 31) && (long)T * HQ < (1l << 31) - 4, "hils_paged_attn: sizes too large for the grid");
   HILS_REQUIRE(q_batch_stride % 8 == 0 && q_token_stride % 8 == 0 && q_head_stride % 8 == 0 && (uintptr_t)q % 16 == 0,
                "hils_paged_attn: q's strides and address must be multiples of 16 bytes");
+  HILS_REQUIRE((uintptr_t)k_pages % 16 == 0 && (uintptr_t)v_pages % 16 == 0 && (uintptr_t)workspace % 16 == 0,
+               "hils_paged_attn: pages and workspace must lie at multiples of 16 bytes");
+  HILS_REQUIRE((uintptr_t)o % 8 == 0 && (uintptr_t)lse % 4 == 0, "hils_paged_attn: o must lie at a multiple of 8 bytes, lse of 4 bytes");
   const PagedPlan pl = paged_plan(B, T, HQ, H, D, window, max_pages);
   const long rows = (long)B * T * HQ;
   HILS_REQUIRE((long)pl.n_blk * pl.vs * pl.n_split * H * B < (1l << 31) - 8, "hils_paged_attn: sizes too large for the grid");

@@ -476,7 +476,8 @@ int hils_rotary(const void* q, const void* k, void* q_out, void* k_out, const vo
  *
  * hils_paged_append: keys and values (B,T,H,D) of the last T tokens (slots length - T ..) into their pages, and q (B,T,HQ,D)
  * into q_out (HQ = 0: none).  With rotary_dim > 0 q and k are rotated as by hils_rotary, at positions (B,T), NULL: the
- * token's slot.  Nothing else of the pages is written.  D a multiple of 16, <= 1024. */
+ * token's slot.  Nothing else of the pages is written.  D a multiple of 16, <= 1024.  q, k, v, q_out and the pages lie at
+ * multiples of 16 bytes. */
 int hils_paged_append(const void* q, const void* k, const void* v, void* q_out, void* k_pages, void* v_pages,
                       const int32_t* page_table, const int32_t* lengths, const void* positions, const void* inv_freq,
                       size_t q_batch_stride, size_t q_token_stride, size_t q_head_stride, size_t k_batch_stride,
@@ -492,7 +493,8 @@ int hils_paged_append(const void* q, const void* k, const void* v, void* q_out, 
  * at a chunk's last position.  A token with a parent that is no earlier token, and those that follow it, see nothing (the
  * padding of a ragged batch of trees).  q (B,T,HQ,D) with any strides (multiples of 8 elements); o (B,T,HQ,D) bf16, lse
  * (B,T,HQ) fp32 in natural-log units; rows that see nothing: o = 0, lse = -inf.  What a row does not see does not reach
- * it, whatever lies there.  D in {64,128}, any HQ/H, T <= 256 with parents, sm_scale > 0.
+ * it, whatever lies there.  D in {64,128}, any HQ/H, T <= 256 with parents, sm_scale > 0.  q, k_pages, v_pages and workspace
+ * lie at multiples of 16 bytes, o at one of 8.
  * workspace: hils_paged_attn_workspace bytes (0: none): shares of the keys that several workgroups have are added up there. */
 size_t hils_paged_attn_workspace(int B, int T, int HQ, int H, int D, int window, int max_pages);
 int hils_paged_attn(const void* q, const void* k_pages, const void* v_pages, const int32_t* page_table,

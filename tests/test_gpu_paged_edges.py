@@ -33,3 +33,14 @@ def test_append_leaves_short_sequences_alone(pkg, dev, heads, T, turned):
             want_k[page, :, slot % 64], want_v[page, :, slot % 64] = turned_k[b, t], v[b, t]
     pkg.paged_append(k, v, kp, vp, table, ln, inv_freq=inv if turned else None)
     assert torch.equal(kp, want_k) and torch.equal(vp, want_v)
+
+
+def test_attention_refuses_pages_between_its_loads(pkg, dev):
+    """(refused on the host: no kernel runs)"""
+    note("pools that begin between two multiples of 16 bytes")
+    whole = torch.zeros(9 * 2 * 64 * 64 + 1, device=dev).bfloat16()
+    odd, even = whole[1:].view(9, 2, 64, 64), whole[:-1].view(9, 2, 64, 64)
+    q, table = torch.zeros(1, 1, 4, 64, device=dev).bfloat16(), torch.zeros(1, 4, device=dev, dtype=torch.int32)
+    for k, v in ((odd, even), (even, odd)):
+        with pytest.raises(RuntimeError, match="multiples of 16 bytes"):
+            pkg.paged_flex_attn(q, k, v, table, 100, 64)

@@ -1,0 +1,29 @@
+"""What the operators on a paged cache promise for calls that never reach a kernel, without a GPU: refusals of the C ABI, of
+the layer and of autograd's modes."""
+import ctypes
+
+import pytest
+import torch
+
+A = 1 << 20  # an address that is never read: every call is refused before a launch
+
+
+def at(byte):
+    return ctypes.c_void_p(A + byte)
+
+
+def test_attention_refuses_buffers_between_its_loads(pkg):
+    """Pages are read, shares and outputs written, in pieces of 16 and 8 bytes."""
+    from hils_attention_amd.ops import _cabi
+    lib = _cabi.load()
+    need = lib.hils_paged_attn_workspace(1, 1, 4, 2, 64, 1 << 20, 4096)
+    assert need > 0
+
+    def call(k=0, v=0, o=0, lse=0, ws=0):
+        rc = lib.hils_paged_attn(at(0), at(k), at(v), at(0), None, None, at(o), at(lse), at(ws), need, 512, 256, 64, 1, 1, 4, 2, 64,
+                                 4096, 9, 1 << 18, 0, 1 << 20, 1, 1, 0.1, None)
+        return rc, lib.hils_last_error().decode()
+
+    for kw in ({"k": 2}, {"k": 8}, {"v": 2}, {"v": 4}, {"ws": 4}, {"ws": 8}, {"o": 2}, {"o": 4}, {"lse": 2}):
+        rc, text = call(**kw)
+        assert rc == 1 and "must lie at" in text, (kw, rc, text)
