@@ -431,8 +431,8 @@ class HiLSPagedLayer:
     def draft(self, key_states, value_states, parents=None, q=None, **rotary):
         """Append T tokens (B, T, H, D) on trial: nothing is pooled, the length stays.  ``parents``: for every token the
         drafted one that it follows, an earlier one, or -1 for the last token of the sequence; T or (B, T) ints, on the host
-        (a tensor on the GPU is copied there, which waits for it); None: each follows the one before.  Rotation as in
-        ``update``, at the positions the tokens' depths give them."""
+        (a tensor on the GPU is copied there, which waits for it); None: each follows the one before.  T <= 256 with
+        ``parents``.  Rotation as in ``update``, at the positions the tokens' depths give them."""
         assert not self.drafted, "tokens are on trial: accept() first"
         B, T = key_states.shape[:2]
         assert T > 0, "draft() needs a token"
@@ -440,6 +440,7 @@ class HiLSPagedLayer:
         if parents is not None:
             parents = torch.as_tensor(parents).to("cpu", torch.int64)
             assert tuple(parents.shape) in ((T,), (B, T)), f"parents {tuple(parents.shape)} for {T} tokens"
+            assert T <= 256, f"draft: a tree has at most 256 tokens (got {T})"  # (what paged_flex_attn takes)
             rows = parents.view(-1, T).tolist()
             if any(not -1 <= p < t for row in rows for t, p in enumerate(row)):
                 raise ValueError("draft: a token's parent is an earlier drafted token or -1")

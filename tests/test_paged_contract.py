@@ -27,3 +27,22 @@ def test_attention_refuses_buffers_between_its_loads(pkg):
     for kw in ({"k": 2}, {"k": 8}, {"v": 2}, {"v": 4}, {"ws": 4}, {"ws": 8}, {"o": 2}, {"o": 4}, {"lse": 2}):
         rc, text = call(**kw)
         assert rc == 1 and "must lie at" in text, (kw, rc, text)
+
+
+def _books(c):
+    return c.seq_len, c.drafted, c.page_table.clone().tolist(), list(c.free_pages), [list(p) for p in c._pages], list(c._users)
+
+
+def test_draft_refuses_a_tree_that_the_attention_does_not_take(pkg):
+    c = pkg.HiLSPagedLayer(num_pages=24, batch=2, max_pages_per_seq=12, num_kv_heads=1, head_dim=16, device="cpu")
+    z = lambda t: torch.ones(2, t, 1, 16, dtype=torch.bfloat16)
+    c.update(z(10), z(10))
+    was = _books(c)
+    with pytest.raises(AssertionError, match="at most 256"):
+        c.draft(z(257), z(257), parents=list(range(-1, 256)))
+    assert _books(c) == was
+    c.draft(z(256), z(256), parents=list(range(-1, 255)))
+    c.truncate(10)
+    c.draft(z(300), z(300))  # (a chain may be longer)
+    c.truncate(10)
+    assert _books(c)[0] == 10 and len(c.free_pages) == 22
