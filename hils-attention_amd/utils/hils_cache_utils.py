@@ -526,17 +526,19 @@ class HiLSPagedLayer:
             self.prior_hm[to, :, :n] = self.prior_hm[fr, :, :n]
 
     def compact(self):
-        """Move the pages in use to the front of the pools; returns their number (the pools behind it are free)."""
+        """Move the pages in use to the front of the pools, or of the part of them that ``page_order`` gave the layer; returns
+        their number (the layer's pages behind are free)."""
         used = [p for p in range(self.num_pages) if self._users[p]]
+        own = sorted(used + self.free_pages)
         n = len(used)
-        holes = [p for p in range(n) if not self._users[p]]
-        moved = dict(zip([p for p in used if p >= n], holes))
+        front = set(own[:n])
+        moved = dict(zip([p for p in used if p not in front], [p for p in own[:n] if not self._users[p]]))
         if moved:
             copy_pages(self._pools(), list(moved.keys()), list(moved.values()))
             for old, new in moved.items():
                 self._users[new], self._users[old] = self._users[old], 0
             self._pages = [[moved.get(p, p) for p in pages] for pages in self._pages]
-            self.free_pages = list(range(self.num_pages - 1, n - 1, -1))
+            self.free_pages = own[:n - 1:-1]
             mapped = max(len(p) for p in self._pages)
             self.page_table[:, :mapped] = torch.tensor(self._pages, dtype=torch.int32, device=self.page_table.device)
         return n

@@ -46,3 +46,31 @@ def test_draft_refuses_a_tree_that_the_attention_does_not_take(pkg):
     c.draft(z(300), z(300))  # (a chain may be longer)
     c.truncate(10)
     assert _books(c)[0] == 10 and len(c.free_pages) == 22
+
+
+@pytest.mark.parametrize("order", [[7, 1, 4, 9, 3, 8], [5, 3, 1, 0, 2, 4, 9, 8, 7, 6]])
+def test_compact_keeps_to_the_pages_of_the_layer(pkg, monkeypatch, order):
+    """A layer that has only some of the pools' pages moves nothing onto the others and hands none of them out."""
+    import hils_attention_amd.utils.hils_cache_utils as utils
+
+    def copy(pools, src, dst):
+        for pool in pools:
+            pool[dst] = pool[src].clone()
+
+    monkeypatch.setattr(utils, "copy_pages", copy)
+    c = pkg.HiLSPagedLayer(num_pages=10, batch=2, max_pages_per_seq=3, num_kv_heads=1, head_dim=16, device="cpu", page_order=order)
+    others = [p for p in range(10) if p not in order]
+    c.k_pages[others] = c.v_pages[others] = 7.0
+    gen = torch.Generator().manual_seed(1)
+    z = lambda t: torch.randn(2, t, 1, 16, generator=gen).bfloat16()
+    c.update(z(50), z(50))
+    c.draft(z(100), z(100))
+    c.truncate(50)
+    k, v = c.gather_contiguous()
+    assert c.compact() == 2
+    assert c._pages == [[p] for p in c.page_table[:, 0].tolist()] and sorted(sum(c._pages, [])) == sorted(order)[:2]
+    assert sorted(c.free_pages) == sorted(order)[2:] and c.free_pages[-1] == min(c.free_pages)
+    assert all(torch.equal(x, y) for x, y in zip(c.gather_contiguous(), (k, v)))
+    assert (c.k_pages[others] == 7).all() and (c.v_pages[others] == 7).all()
+    c.free()
+    assert c.compact() == 0 and sorted(c.free_pages) == sorted(order)
