@@ -70,9 +70,10 @@ def copy_pages(pools, src, dst):
     pools = list(pools)
     if not isinstance(src, torch.Tensor) or not isinstance(dst, torch.Tensor):
         src, dst = [int(x) for x in src], [int(x) for x in dst]
-        pairs = [(a, b) for a, b in zip(src, dst) if a != b]
         if len(src) != len(dst):
             raise ValueError(f"copy_pages: {len(src)} sources and {len(dst)} destinations")
+        n = pools[0].shape[0] if pools and pools[0].dim() else 0
+        pairs = [(a, b) for a, b in zip(src, dst) if a != b and 0 <= a < n and 0 <= b < n]  # (the others are left out)
         written = [b for _, b in pairs]
         if len(set(written)) < len(written) or set(written) & {a for a, _ in pairs}:
             raise ValueError("copy_pages: a page that is written is in another pair too")

@@ -74,3 +74,15 @@ def test_compact_keeps_to_the_pages_of_the_layer(pkg, monkeypatch, order):
     assert (c.k_pages[others] == 7).all() and (c.v_pages[others] == 7).all()
     c.free()
     assert c.compact() == 0 and sorted(c.free_pages) == sorted(order)
+
+
+def test_copied_pairs_that_are_left_out_are_in_no_ones_way(pkg):
+    """Of pairs given as numbers only those that move a page have to be apart."""
+    pool = torch.zeros(5, 8)
+    for src, dst in (([0, 1, 2], [-1, -1, 3]), ([5, 6, 2], [3, 3, 3]), ([0, -1, 9], [1, 0, 0]), ([2, 2, 0], [2, 2, 2]),
+                     ([0, 7], [2, 2])):
+        with pytest.raises(RuntimeError, match="no CPU path"):  # (what pairs that are taken end in here)
+            pkg.copy_pages([pool], src, dst)
+    for src, dst in (([0, 1], [4, 4]), ([0, 4], [4, 3])):
+        with pytest.raises(ValueError, match="another pair"):
+            pkg.copy_pages([pool], src, dst)
