@@ -868,15 +868,19 @@ void same_device(const char* name, const Tensor& like, std::initializer_list<con
       throw std::runtime_error(c10::str(name, ": tensors on ", like.device().str(), " and ", t->device().str()));
 }
 
+// Elements between the sequences, tokens or heads of (B, T, heads, D); of a single one any number is as good (a tensor counts as
+// contiguous whatever stands there), and none for a missing tensor.
+size_t row_stride(const Tensor& t, int64_t dim) { return t.defined() && t.size(dim) > 1 ? (size_t)t.stride(dim) : 0; }
+#define ROW_STRIDES(t) row_stride(t, 0), row_stride(t, 1), row_stride(t, 2)
+
 // (B, T, heads, D) rows the kernels can read where they are: contiguous features, everything at multiples of 16 bytes
 Tensor strided_rows(const Tensor& t) {
-  const bool fits = t.stride(3) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 && t.stride(2) % 8 == 0 &&
-                    t.stride(0) >= 0 && t.stride(1) >= 0 && t.stride(2) >= 0 && (uintptr_t)t.const_data_ptr() % 16 == 0;
+  const bool fits = t.stride(3) == 1 && row_stride(t, 0) % 8 == 0 && row_stride(t, 1) % 8 == 0 && row_stride(t, 2) % 8 == 0 &&
+                    (uintptr_t)t.const_data_ptr() % 16 == 0;
   if (fits) return t;
   const Tensor c = t.contiguous();
   return (uintptr_t)c.const_data_ptr() % 16 ? c.clone(at::MemoryFormat::Contiguous) : c;
 }
-#define ROW_STRIDES(t) (size_t)(t).stride(0), (size_t)(t).stride(1), (size_t)(t).stride(2)
 
 struct Turn {
   Tensor positions, inv_freq;
@@ -922,8 +926,7 @@ std::tuple<Tensor, Tensor> rotary_forward(const Tensor& q, const Tensor& k, cons
   const Tensor qs = strided_rows(q), ks = k.defined() ? strided_rows(k) : Tensor();
   const Tensor pos = c.positions.defined() ? c.positions.contiguous() : Tensor();
   HILS_CALL(hils_rotary, cptr(qs), cptr(ks), mptr(qo), mptr(ko), cptr(pos), cptr(c.inv_freq), ROW_STRIDES(qs),
-            (size_t)(H ? ks.stride(0) : 0), (size_t)(H ? ks.stride(1) : 0), (size_t)(H ? ks.stride(2) : 0), i32(B), i32(T),
-            i32(HQ), i32(H), i32(D), i32(2 * c.inv_freq.numel()), i32(c.interleaved),
+            ROW_STRIDES(ks), i32(B), i32(T), i32(HQ), i32(H), i32(D), i32(2 * c.inv_freq.numel()), i32(c.interleaved),
             (int)(pos.defined() && pos.scalar_type() == at::kLong), (int)(pos.defined() && pos.dim() == 2), i32(c.first),
             (int)(c.inv_freq.scalar_type() == at::kDouble), (float)c.scale, (float)sign);
   return {qo, ko};
@@ -1047,8 +1050,7 @@ Tensor paged_append(const Tensor& k, const Tensor& v, const Tensor& k_pages, con
   const Tensor ks = strided_rows(k), vs = strided_rows(v), qs = HQ ? strided_rows(q) : Tensor();
   const Tensor pos = c.positions.defined() ? c.positions.contiguous() : Tensor();
   HILS_CALL(hils_paged_append, cptr(qs), cptr(ks), cptr(vs), HQ ? mptr(qo) : nullptr, mptr(k_pages), mptr(v_pages), iptr(table),
-            iptr(p.lengths), cptr(pos), cptr(c.inv_freq), (size_t)(HQ ? qs.stride(0) : 0), (size_t)(HQ ? qs.stride(1) : 0),
-            (size_t)(HQ ? qs.stride(2) : 0), ROW_STRIDES(ks), ROW_STRIDES(vs), i32(B), i32(T), i32(HQ), i32(H), i32(D),
+            iptr(p.lengths), cptr(pos), cptr(c.inv_freq), ROW_STRIDES(qs), ROW_STRIDES(ks), ROW_STRIDES(vs), i32(B), i32(T), i32(HQ), i32(H), i32(D),
             i32(c.inv_freq.defined() ? 2 * c.inv_freq.numel() : 0), (int)interleaved,
             (int)(pos.defined() && pos.scalar_type() == at::kLong),
             (int)(c.inv_freq.defined() && c.inv_freq.scalar_type() == at::kDouble), i32(p.max_pages), i32(p.pages),

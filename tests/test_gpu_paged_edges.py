@@ -44,3 +44,31 @@ def test_attention_refuses_pages_between_its_loads(pkg, dev):
     for k, v in ((odd, even), (even, odd)):
         with pytest.raises(RuntimeError, match="multiples of 16 bytes"):
             pkg.paged_flex_attn(q, k, v, table, 100, 64)
+
+
+def _single(x, strides):
+    """x (1,1,1,D) with any strides of its dimensions of one."""
+    whole = torch.zeros(4096, dtype=x.dtype, device=x.device)
+    y = whole.as_strided(x.shape, (*strides, 1))
+    return y.copy_(x)
+
+
+@pytest.mark.parametrize("strides", [(65, 65, 65), (3, 129, 64), (0, 1, 2), (64, 64, 64)])
+def test_strides_of_single_rows_do_not_matter(pkg, dev, strides):
+    """One token of one head, cut from rows of an odd width: torch calls it contiguous whatever its strides are."""
+    note(f"single rows with strides {strides}")
+    gen = torch.Generator().manual_seed(3)
+    kp, vp, table = ref.cache(gen, 1, 3, 1, 64, dev)
+    q, k, v = (torch.randn(1, 1, 1, 64, generator=gen).bfloat16().to(dev) for _ in range(3))
+    inv, _ = pkg.rotary_frequencies(64, device=dev)
+    runs = []
+    for cut in (lambda x: x, lambda x: _single(x, strides)):
+        k1, v1 = kp.clone(), vp.clone()
+        a, b = cut(q).requires_grad_(), cut(k).requires_grad_()
+        turned = pkg.rotary_embedding(a, b, 70, inv)
+        grads = torch.autograd.grad(turned, [a, b], [cut(v), cut(q)])
+        new = pkg.paged_append(cut(k), cut(v), k1, v1, table, 100, q=cut(q), inv_freq=inv)
+        out = pkg.paged_flex_attn(cut(q), k1, v1, table, 100, 512)
+        runs.append([x.detach() for x in (*turned, *grads, new, *out, k1, v1)])
+    assert all(torch.equal(x, y) for x, y in zip(*runs))
+    ref.check_attention(out, ref.attend(q, k1, v1, table, 100, 512))
