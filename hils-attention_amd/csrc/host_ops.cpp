@@ -873,6 +873,11 @@ void same_device(const char* name, const Tensor& like, std::initializer_list<con
 size_t row_stride(const Tensor& t, int64_t dim) { return t.defined() && t.size(dim) > 1 ? (size_t)t.stride(dim) : 0; }
 #define ROW_STRIDES(t) row_stride(t, 0), row_stride(t, 1), row_stride(t, 2)
 
+// A tensor that a kernel has written in place: autograd nodes that keep it notice, as with torch's own in-place operations.
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // (B, T, heads, D) rows the kernels can read where they are: contiguous features, everything at multiples of 16 bytes
 Tensor strided_rows(const Tensor& t) {
   const bool fits = t.stride(3) == 1 && row_stride(t, 0) % 8 == 0 && row_stride(t, 1) % 8 == 0 && row_stride(t, 2) % 8 == 0 &&
@@ -1055,6 +1060,8 @@ Tensor paged_append(const Tensor& k, const Tensor& v, const Tensor& k_pages, con
             (int)(pos.defined() && pos.scalar_type() == at::kLong),
             (int)(c.inv_freq.defined() && c.inv_freq.scalar_type() == at::kDouble), i32(p.max_pages), i32(p.pages),
             i32(p.seq_len), (float)scale);
+  written(k_pages);
+  written(v_pages);
   return qo;
 }
 
@@ -1106,6 +1113,8 @@ void paged_accept(const Tensor& k_pages, const Tensor& v_pages, const Tensor& ta
   const Tensor way = path.contiguous();
   HILS_CALL(hils_paged_accept, mptr(k_pages), mptr(v_pages), iptr(table), iptr(p.lengths), iptr(way), i32(p.B), i32(n), i32(p.H),
             i32(p.D), i32(p.max_pages), i32(p.pages), i32(p.seq_len));
+  written(k_pages);
+  written(v_pages);
 }
 
 void copy_pages(const std::vector<Tensor>& pools, const Tensor& src, const Tensor& dst) {
@@ -1134,6 +1143,7 @@ void copy_pages(const std::vector<Tensor>& pools, const Tensor& src, const Tenso
   const Tensor from = src.contiguous(), to = dst.contiguous();
   HILS_CALL(hils_copy_pages, at_, size, cptr(from), cptr(to), (int)pools.size(), i32(from.numel()), i32(pools[0].size(0)),
             (int)(dt == at::kLong));
+  for (const Tensor& t : pools) written(t);
 }
 
 }  // namespace

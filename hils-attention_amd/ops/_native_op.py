@@ -47,3 +47,36 @@ class NativeOp(torch.autograd.Function):
             for i, g in zip(wanted, found):
                 result[i] = g
         return tuple(result)
+
+
+def bare(*tensors):
+    """A call on these tensors (or None) has to give its result and nothing else: no trace, tangent, transform or gradient."""
+    if _is_tracing() or forward_ad._current_level >= 0 or _in_transform():
+        return False
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            return not torch.is_grad_enabled()
+    return True
+
+
+class InferenceOp(torch.autograd.Function):
+    """Base class of an operator without a backward: a subclass defines ``label``, ``native(*args)``, ``forward(ctx, *args)``
+    as ``return <subclass>.native(*args)`` and, if it writes to arguments in place, which (``written``).  Its function calls
+    ``native`` itself where that is all that is wanted; ``apply`` is for the other calls: a trace records them as a node,
+    tangents and function transforms are refused, a gradient through the result is refused when it is asked for, and one
+    through what is written, which would miss it, at once."""
+
+    label, written = "", slice(0)
+
+    @classmethod
+    def apply(cls, *args):
+        if torch.is_grad_enabled() and any(t.requires_grad for t in args[cls.written]):
+            raise RuntimeError(f"{cls.label} is an inference operator: what it writes to must not require gradients")
+        if forward_ad._current_level >= 0 and not _in_transform() and any(
+                isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in args):
+            raise NotImplementedError(f"{cls.label} is an inference operator: its jvp is not supported")
+        return super().apply(*args)
+
+    @classmethod
+    def refuse(cls):
+        raise RuntimeError(f"{cls.label} is an inference operator: its backward is not supported")

@@ -3,28 +3,69 @@
 The layouts are those of ``HiLSPagedLayer`` and ``paged_hils_attend``: k_pages, v_pages (num_pages, H, 64, D) bf16,
 page_table (B, max_pages) int32 (entries outside the pool: not mapped).  Lengths are an int for all sequences or an int32
 tensor (B,) on the GPU; a sequence shorter than the T tokens of a call takes no part in it.  Everything runs on the current
-stream and synchronises nothing; inference only.
+stream and synchronises nothing; inference only: a backward through an output, tangents and pages that require gradients
+where they are written are refused.
 """
 import torch
 
 from . import _cabi
+from ._native_op import InferenceOp, bare
 
 
-class _NoBackward(torch.autograd.Function):
-    """Outputs of an inference operator whose inputs want gradients: a backward through them is refused."""
+class _PagedAppend(InferenceOp):
+    label, written = "paged_append", slice(2, 4)
 
     @staticmethod
-    def forward(ctx, name, call, *inputs):
-        ctx.name = name
-        return call()
+    def native(*args):
+        return _cabi.host().paged_append(*args)
+
+    @staticmethod
+    def forward(ctx, *args):
+        return _PagedAppend.native(*args)
 
     @staticmethod
     def backward(ctx, *grads):
-        raise RuntimeError(f"{ctx.name} is an inference operator: its backward is not supported")
+        _PagedAppend.refuse()
 
 
-def _inference(name, call, *inputs):
-    return _NoBackward.apply(name, call, *inputs) if torch.is_grad_enabled() else call()
+class _PagedFlexAttn(InferenceOp):
+    label = "paged_flex_attn"
+
+    @staticmethod
+    def native(*args):
+        return _cabi.host().paged_flex_attn(*args)
+
+    @staticmethod
+    def forward(ctx, *args):
+        return _PagedFlexAttn.native(*args)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        _PagedFlexAttn.refuse()
+
+
+class _PagedAccept(InferenceOp):
+    label, written = "paged_accept", slice(0, 2)
+
+    @staticmethod
+    def native(*args):
+        return _cabi.host().paged_accept(*args)
+
+    @staticmethod
+    def forward(ctx, *args):
+        return _PagedAccept.native(*args)
+
+
+class _CopyPages(InferenceOp):
+    label, written = "copy_pages", slice(2, None)
+
+    @staticmethod
+    def native(src, dst, *pools):
+        return _cabi.host().copy_pages(pools, src, dst)
+
+    @staticmethod
+    def forward(ctx, *args):
+        return _CopyPages.native(*args)
 
 
 def paged_append(k, v, k_pages, v_pages, page_table, seq_len, q=None, inv_freq=None, positions=None, interleaved=False,
@@ -33,9 +74,7 @@ def paged_append(k, v, k_pages, v_pages, page_table, seq_len, q=None, inv_freq=N
     page is not mapped, and sequences shorter than T, are left out.  With ``inv_freq`` the keys, and q (B,T,H_q,D) if given, are rotated on the way as by
     ``rotary_embedding``, at ``positions`` (B,T) or, without them, at the tokens' slots.  Returns the rotated q or None."""
     args = (k, v, k_pages, v_pages, page_table, seq_len, q, inv_freq, positions, bool(interleaved), float(scale))
-    if k.requires_grad or v.requires_grad or (q is not None and q.requires_grad):
-        return _inference("paged_append", lambda: _cabi.host().paged_append(*args), q, k, v)
-    return _cabi.host().paged_append(*args)
+    return (_PagedAppend.native if bare(k, v, k_pages, v_pages, q) else _PagedAppend.apply)(*args)
 
 
 def paged_flex_attn(q, k_pages, v_pages, page_table, seq_len, window_size, parents=None, mask_lmk=True,
@@ -50,16 +89,14 @@ def paged_flex_attn(q, k_pages, v_pages, page_table, seq_len, window_size, paren
     Returns o (B,T,H_q,D) bf16 and lse (B,T,H_q) fp32, natural log; rows that see nothing: 0 and -inf.  The same call gives
     the same bits; a sequence's last bits may depend on how many others, and how long ones, are in the batch."""
     args = (q, k_pages, v_pages, page_table, seq_len, int(window_size), parents, bool(mask_lmk), bool(expand_to_chunk), sm_scale)
-    if q.requires_grad or k_pages.requires_grad or v_pages.requires_grad:
-        return _inference("paged_flex_attn", lambda: _cabi.host().paged_flex_attn(*args), q, k_pages, v_pages)
-    return _cabi.host().paged_flex_attn(*args)
+    return (_PagedFlexAttn.native if bare(q, k_pages, v_pages) else _PagedFlexAttn.apply)(*args)
 
 
 def paged_accept(k_pages, v_pages, page_table, base_len, path):
     """Move accepted drafts to the front: keys and values at slots ``base_len + path[b][i]`` go to ``base_len + i``.
     ``path`` int32 (B,n) on the GPU, growing strictly; the first entry that does not (-1, say) ends it.  The pages from slot
     ``base_len`` on must be the sequence's own."""
-    _cabi.host().paged_accept(k_pages, v_pages, page_table, base_len, path)
+    (_PagedAccept.native if bare(k_pages, v_pages) else _PagedAccept.apply)(k_pages, v_pages, page_table, base_len, path)
 
 
 def copy_pages(pools, src, dst):
@@ -79,4 +116,4 @@ def copy_pages(pools, src, dst):
             raise ValueError("copy_pages: a page that is written is in another pair too")
         dev = pools[0].device if pools else None
         src, dst = (torch.tensor(x, dtype=torch.int64, device=dev) for x in (src, dst))
-    _cabi.host().copy_pages(pools, src, dst)
+    (_CopyPages.native if bare(*pools) else _CopyPages.apply)(src, dst, *pools)

@@ -72,3 +72,27 @@ def test_strides_of_single_rows_do_not_matter(pkg, dev, strides):
         runs.append([x.detach() for x in (*turned, *grads, new, *out, k1, v1)])
     assert all(torch.equal(x, y) for x, y in zip(*runs))
     ref.check_attention(out, ref.attend(q, k1, v1, table, 100, 512))
+
+
+def test_autograd_notices_what_is_written(pkg, dev):
+    """A backward that needs what the pages held before is refused, as after torch's own writes in place."""
+    note("pages kept for a backward, then written")
+    gen = torch.Generator().manual_seed(4)
+    kp, vp, table = ref.cache(gen, 1, 2, 2, 64, dev)
+    k = torch.randn(1, 2, 2, 64, generator=gen).bfloat16().to(dev)
+    path = torch.tensor([[1]], dtype=torch.int32, device=dev)
+    for call, pools in ((lambda: pkg.paged_append(k, k, kp, vp, table, 10), (kp, vp)), (lambda: pkg.paged_accept(kp, vp, table, 3, path), (kp, vp)),
+                        (lambda: pkg.copy_pages([kp, vp], [0], [1]), (kp, vp))):
+        for pool in pools:
+            x = torch.ones_like(pool).requires_grad_()
+            loss = (x * pool).sum()
+            call()
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                loss.backward()
+    with torch.inference_mode():
+        kept = torch.zeros_like(kp), torch.zeros_like(vp)
+    pkg.paged_append(k, k, *kept, table, 10)  # (tensors of inference mode have nothing that could notice)
+    with torch.inference_mode():
+        pkg.paged_append(k, k, *kept, table, 12)
+        pkg.paged_append(k, k, kp, vp, table, 12)
+    assert (kept[0] != 0).any(-1).sum() == 8

@@ -1,9 +1,11 @@
 """What the operators on a paged cache promise for calls that never reach a kernel, without a GPU: refusals of the C ABI, of
 the layer and of autograd's modes."""
 import ctypes
+import warnings
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 A = 1 << 20  # an address that is never read: every call is refused before a launch
 
@@ -86,3 +88,111 @@ def test_copied_pairs_that_are_left_out_are_in_no_ones_way(pkg):
     for src, dst in (([0, 1], [4, 4]), ([0, 4], [4, 3])):
         with pytest.raises(ValueError, match="another pair"):
             pkg.copy_pages([pool], src, dst)
+
+
+def _put(to, x):
+    """A write behind torch's back, as the native operators write."""
+    x = x.detach().contiguous()
+    ctypes.memmove(to.data_ptr(), x.data_ptr(), x.numel() * x.element_size())
+
+
+class _StandIn:
+    """The native operators in place of which something simple is computed on the same arguments."""
+
+    def paged_append(self, k, v, k_pages, v_pages, table, seq_len, q, inv_freq, positions, interleaved, scale):
+        _put(k_pages, k)
+        _put(v_pages, v)
+        if q is None:
+            return None
+        out = torch.empty_like(q)
+        _put(out, q.detach() * scale)
+        return out
+
+    def paged_flex_attn(self, q, k_pages, *_):
+        out = torch.empty_like(q)
+        _put(out, q.detach() + k_pages.detach().flatten()[:1])
+        return out, out.float().sum(-1)
+
+    def paged_accept(self, k_pages, v_pages, table, base, path):
+        _put(k_pages, k_pages.detach() * 3)
+
+    def copy_pages(self, pools, src, dst):
+        for pool in pools:
+            _put(pool, pool.detach() + 1)
+
+
+def _calls(pkg):
+    """(name, call on (k, q, k_pages, v_pages), arguments it writes)"""
+    table = torch.zeros(1, 2, dtype=torch.int32)
+    one = torch.ones(1, dtype=torch.int32)
+    return [("paged_append", lambda k, q, kp, vp: pkg.paged_append(k, k, kp, vp, table, 10, q=q, inv_freq=torch.ones(32), scale=2.0), (2, 3)),
+            ("paged_append", lambda k, q, kp, vp: pkg.paged_append(k, k, kp, vp, table, 10), (2, 3)),
+            ("paged_flex_attn", lambda k, q, kp, vp: pkg.paged_flex_attn(q, kp, vp, table, 10, 64)[0], ()),
+            ("copy_pages", lambda k, q, kp, vp: pkg.copy_pages([kp, vp], one, one), (2, 3)),
+            ("paged_accept", lambda k, q, kp, vp: pkg.paged_accept(kp, vp, table, 3, torch.zeros(1, 2, dtype=torch.int32)), (2, 3))]
+
+
+def _tensors(seed):
+    gen = torch.Generator().manual_seed(seed)
+    return [torch.randn(*s, generator=gen).bfloat16() for s in ((1, 2, 2, 64), (1, 2, 4, 64), (4, 2, 64, 64), (4, 2, 64, 64))]
+
+
+def _stand_in(monkeypatch):
+    from hils_attention_amd.ops import _cabi
+    monkeypatch.setattr(_cabi, "host", lambda: _StandIn())
+
+
+def test_a_trace_records_the_calls(pkg, monkeypatch):
+    _stand_in(monkeypatch)
+    calls = [c for _, c, _ in _calls(pkg)]
+
+    def step(k, q, kp, vp):
+        q = calls[0](k, q, kp, vp)
+        for call in (calls[1], calls[3], calls[4]):
+            call(k, q, kp, vp)
+        return calls[2](k, q, kp, vp)
+
+    with warnings.catch_warnings():
+        warnings.simplefilter("ignore")
+        traced = torch.jit.trace(step, tuple(_tensors(1)), check_trace=False)
+    one, two = _tensors(2), _tensors(2)
+    assert torch.equal(traced(*one), step(*two)) and not torch.equal(one[2], _tensors(2)[2])
+    assert all(torch.equal(x, y) for x, y in zip(one, two))
+
+
+def test_tangents_and_transforms_are_refused(pkg, monkeypatch):
+    _stand_in(monkeypatch)
+    args = _tensors(1)
+    for name, call, _ in _calls(pkg):
+        given = [2, 3] if name in ("copy_pages", "paged_accept") else [1, 2, 3] if name == "paged_flex_attn" else [0, 2, 3]
+        for i in given:
+            was = [x.clone() for x in args]
+            with forward_ad.dual_level():
+                duals = list(args)
+                duals[i] = forward_ad.make_dual(args[i], torch.ones_like(args[i]))
+                with pytest.raises(NotImplementedError, match=f"{name} .* jvp"):
+                    call(*duals)
+            with pytest.raises(RuntimeError):
+                torch.vmap(lambda x: call(*args[:i], x, *args[i + 1:]))(args[i].unsqueeze(0))
+            assert all(torch.equal(x, y) for x, y in zip(args, was))
+        with forward_ad.dual_level():
+            call(*args)  # (no tangent: nothing is lost)
+
+
+def test_pages_that_require_gradients_are_not_written(pkg, monkeypatch):
+    _stand_in(monkeypatch)
+    for name, call, written in _calls(pkg):
+        for i in written:
+            args = _tensors(1)
+            args[i].requires_grad_()
+            was = [x.detach().clone() for x in args]
+            with pytest.raises(RuntimeError, match=f"{name} .* must not require gradients"):
+                call(*args)
+            assert all(torch.equal(x, y) for x, y in zip(args, was))
+            with torch.no_grad():
+                call(*args)
+        if not written:
+            args = _tensors(1)
+            out = call(*[x.requires_grad_() for x in args])
+            with pytest.raises(RuntimeError, match=f"{name} is an inference operator"):
+                out.float().sum().backward()
