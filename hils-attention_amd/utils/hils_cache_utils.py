@@ -23,17 +23,21 @@ import torch
 
 try:  # imported as part of the package ...
     from ..ops import _cabi
+    from ..ops._native_op import bare
     from ..ops.chunk_attn_pool_tilelang import chunk_attn_pool, chunk_mean_pool
     from ..ops.hils_fwd_bwd_head import HiLS_block_M_head
     from ..ops.hils_glue import chunk_weights, decode_step, topk_chunk_weights
     from ..ops.paged_cache import copy_pages, paged_accept, paged_append, paged_flex_attn
+    from ..ops.rotary import rotary_embedding
     from ..ops.topk_head_softmax import online_softmax_topk_head
 except ImportError:  # ... or with the package directory itself on sys.path (`from utils... import`)
     from ops import _cabi
+    from ops._native_op import bare
     from ops.chunk_attn_pool_tilelang import chunk_attn_pool, chunk_mean_pool
     from ops.hils_fwd_bwd_head import HiLS_block_M_head
     from ops.hils_glue import chunk_weights, decode_step, topk_chunk_weights
     from ops.paged_cache import copy_pages, paged_accept, paged_append, paged_flex_attn
+    from ops.rotary import rotary_embedding
     from ops.topk_head_softmax import online_softmax_topk_head
 
 
@@ -235,7 +239,8 @@ class HiLSPagedLayer:
     free list, so the page order of a sequence is arbitrary.
 
     Sequences may share pages after ``fork``: a page counts its users, returns to the free list when the last one lets go
-    of it, and is copied before a sequence writes on a page that others use too.  ``draft`` appends tokens on trial, in a
+    of it, and is copied before a sequence writes on a page that others use too.  Keys and values that require gradients
+    get them through the pages (``gather_contiguous``, the chunk keys); the attention on the pages itself has no backward.  ``draft`` appends tokens on trial, in a
     chain or a tree; ``local_attend`` and ``hils_attend`` then are for them, and ``accept`` keeps a path of the tree and
     drops the rest.  ``truncate`` and ``free`` give tokens up, ``compact`` gathers the pages in use at the front."""
 
@@ -315,7 +320,7 @@ class HiLSPagedLayer:
         if not who:
             return
         src, dst = [self._pages[b][c] for b in who], self.free_pages[-len(who):]
-        copy_pages(self._pools(), src, dst)
+        self._copy_pages(src, dst)
         dev = self.page_table.device
         self.page_table[torch.tensor(who, device=dev), c] = torch.tensor(dst, dtype=torch.int32, device=dev)
         del self.free_pages[-len(who):]
@@ -358,16 +363,49 @@ class HiLSPagedLayer:
         B, T, H, D = key_states.shape
         S = self.S
         if self.k_pages.is_cuda and self.k_pages.dtype == torch.bfloat16 and D % 16 == 0 and D <= 1024:
-            return paged_append(key_states, value_states, self.k_pages, self.v_pages, self.page_table, b_end, q=q, **rotary)
-        # a cache in a type that the attention does not take is kept all the same
-        assert q is None and not rotary, "the rotation needs a bf16 cache on the GPU"
+            if bare(key_states, value_states, q, self.k_pages, self.v_pages):
+                return paged_append(key_states, value_states, self.k_pages, self.v_pages, self.page_table, b_end, q=q, **rotary)
+            # gradients go through the pages to the keys and values: steps that autograd knows
+            q, key_states = self._rotate(q, key_states, a, **rotary)
+        else:  # a cache in a type that the attention does not take is kept all the same
+            assert q is None and not rotary, "the rotation needs a bf16 cache on the GPU"
         pos = torch.arange(a, b_end, device=self.k_pages.device)
         pages = self.page_table[:, pos // S].long().unsqueeze(-1)        # (B, T, 1)
         slots = (pos % S).view(1, T, 1).expand(B, T, 1)
         hh = torch.arange(H, device=self.k_pages.device).view(1, 1, H)
         self.k_pages[pages, hh, slots] = key_states
         self.v_pages[pages, hh, slots] = value_states
-        return None
+        return q
+
+    @staticmethod
+    def _rotate(q, k, first, inv_freq=None, positions=None, interleaved=False, scale=1.0):
+        if inv_freq is None:
+            assert q is None and positions is None, "q and positions are for the rotation: inv_freq is missing"
+            return None, k
+        at = first if positions is None else positions
+        if q is None:
+            return None, rotary_embedding(k, None, at, inv_freq, interleaved, scale)[0]
+        return rotary_embedding(q, k, at, inv_freq, interleaved, scale)
+
+    def _copy_pages(self, src, dst):
+        pools = self._pools()
+        if bare(*pools):
+            copy_pages(pools, src, dst)
+        else:
+            for pool in pools:
+                pool[dst] = pool[src]
+
+    def _move_drafts(self, path):
+        """Drafted tokens path (B, n) to the front of the drafts' slots."""
+        dev, base, S = self.k_pages.device, self.seq_len, self.S
+        if bare(self.k_pages, self.v_pages):
+            paged_accept(self.k_pages, self.v_pages, self.page_table, base, path.to(dev, torch.int32))
+            return
+        fr = base + path.to(dev)
+        to = base + torch.arange(path.shape[1], device=dev).expand_as(fr)
+        here, there = (self.page_table.long().gather(1, x // S) for x in (fr, to))
+        for pool in (self.k_pages, self.v_pages):
+            pool[there, :, to % S] = pool[here, :, fr % S]
 
     def _check_prior(self, tokens, mu_q):
         """Refuse prior queries that do not go with the chunks that `tokens` tokens complete (before anything is changed)."""
@@ -480,8 +518,7 @@ class HiLSPagedLayer:
                 raise ValueError(f"accept: {way} is no way down the tree of sequence {b}")
         self._check_prior(self.seq_len + n, mu_q)
         if n and not torch.equal(path, torch.arange(n).expand(self.B, n)):
-            paged_accept(self.k_pages, self.v_pages, self.page_table, self.seq_len,
-                         path.to(self.k_pages.device, torch.int32))
+            self._move_drafts(path)
         self.drafted, self._parents, self._parents_dev, self._depth_rows = 0, None, None, None
         self.seq_len += n
         self._keep_pages(self.seq_len)
@@ -534,7 +571,7 @@ class HiLSPagedLayer:
         front = set(own[:n])
         moved = dict(zip([p for p in used if p not in front], [p for p in own[:n] if not self._users[p]]))
         if moved:
-            copy_pages(self._pools(), list(moved.keys()), list(moved.values()))
+            self._copy_pages(list(moved.keys()), list(moved.values()))
             for old, new in moved.items():
                 self._users[new], self._users[old] = self._users[old], 0
             self._pages = [[moved.get(p, p) for p in pages] for pages in self._pages]

@@ -96,3 +96,69 @@ def test_autograd_notices_what_is_written(pkg, dev):
         pkg.paged_append(k, k, *kept, table, 12)
         pkg.paged_append(k, k, kp, vp, table, 12)
     assert (kept[0] != 0).any(-1).sum() == 8
+
+
+@pytest.mark.parametrize("turned", [False, True])
+def test_gradients_through_the_layers_pages(pkg, dev, turned):
+    """Keys and values that want gradients: the cache is that of the direct call, bit for bit, and each gets the gradient of
+    the tokens that are kept, through appends, drafts, forks and compaction."""
+    note(f"a paged layer with gradients, rotated {turned}")
+    B, H, D, first, drafts = 2, 2, 64, 100, 4
+    gen = torch.Generator().manual_seed(5)
+    r = lambda t, h: torch.randn(B, t, h, D, generator=gen).bfloat16().to(dev)
+    k, v, q, dk, dv, dq = r(first, H), r(first, H), r(first, 4), r(drafts, H), r(drafts, H), r(drafts, 4)
+    inv, _ = pkg.rotary_frequencies(D, device=dev)
+    turn = {"inv_freq": inv, "scale": 0.5} if turned else {}
+    layers, outs = [], []
+    leaves = [x.clone().requires_grad_() for x in (k, v, dk, dv)]
+    for kk, vv, dkk, dvv in ((k, v, dk, dv), leaves):
+        c = pkg.HiLSPagedLayer(num_pages=16, batch=B, max_pages_per_seq=4, num_kv_heads=H, head_dim=D, device=dev, page_order=[3, 9, 12, 5, 7, 1, 2, 15])
+        out = [c.update(kk, vv, q=q if turned else None, **turn)]
+        c.fork([1, 1])
+        out.append(c.draft(dkk, dvv, parents=[-1, 0, 0, 2], q=dq if turned else None, **turn))
+        c.accept([0, 2, 3])
+        c.compact()
+        layers.append(c)
+        outs.append(out + list(c.gather_contiguous()) + [c.lmk_hm, c.k_pages, c.v_pages, c.lmk_pages])
+    assert [c._pages for c in layers][0] == layers[1]._pages
+    assert all(x is y is None or torch.equal(x, y) for x, y in zip(*outs))
+    gk, gv = outs[1][2:4]
+    w = [torch.randn(x.shape, generator=gen).bfloat16().to(dev) for x in (gk, gv)]
+    got = torch.autograd.grad([gk, gv], leaves, w)
+    # both sequences are sequence 1's first tokens and their own drafts 0, 2 and 3; a rotation's transpose turns gradients back
+    want = [torch.zeros_like(x) for x in leaves]
+    back = (lambda x, at: pkg.rotary_embedding(x, None, at, inv, scale=0.5)[0]) if turned else (lambda x, at: x)
+    full = back(w[0], -torch.arange(first + 3, device=dev))
+    at = [0, 2, 3]
+    # (of tokens that both sequences have, the sum of the two gradients as one product of bf16 each: two roundings and the sum's)
+    for i, (x, kept) in enumerate(((full, 0), (w[1], 1))):
+        want[i + 2][:, at] = x[:, first:]
+        both = x[:, :first].double().sum(0)
+        err = (got[i][1].double() - both).abs()
+        size = x[:, :first].double().abs().sum(0)
+        if turned and i == 0:  # (rounded before and after the rotation, whose terms are up to twice as large)
+            pair = size[..., : D // 2] + size[..., D // 2:]
+            size = size + 2 * torch.cat([pair, pair], -1)
+        assert (err <= 3 * ref.HALF * size + 1e-30).all()
+        assert (got[i][0] == 0).all()
+        assert torch.equal(got[i + 2], want[i + 2])
+
+
+def test_update_keeps_gradients_of_the_chunk_keys(pkg, dev):
+    note("chunk keys of a paged layer with gradients")
+    gen = torch.Generator().manual_seed(6)
+    c = pkg.HiLSPagedLayer(num_pages=8, batch=2, max_pages_per_seq=3, num_kv_heads=2, head_dim=64, device=dev)
+    k = torch.randn(2, 130, 2, 64, generator=gen).bfloat16().to(dev).requires_grad_()
+    c.update(k, k.detach())
+    (g,) = torch.autograd.grad(c.lmk_hm.float().sum(), k)
+    # the mean of 64 tokens, each weighed 1/64 (exact in bf16); the last two are in no chunk
+    assert (g[:, :128] == 1 / 64).all() and (g[:, 128:] == 0).all()
+    q = torch.randn(2, 1, 4, 64, generator=gen).bfloat16().to(dev)
+    o, lse = c.local_attend(q, 64)
+    with pytest.raises(RuntimeError, match="inference operator"):
+        o.float().sum().backward()
+    with torch.no_grad():
+        c.update(k[:, :1], k[:, :1])
+        c.fork([0, 0])
+        c.update(k[:, :1], k[:, :1])
+    assert c.seq_len == 132
