@@ -1130,11 +1130,11 @@ static PagedPlan paged_choose(int B, int T, int HQ, int H, int D, int window, in
       best.n_split = n_split;
     }
   }
-  // One row block reads a key and a value once.  Where all of them do not fit the last cache, values go past it: 16 sequences of
+  // One row block of 16 reads a key and a value once.  Where all of them do not fit the last cache, values go past it: 16 sequences of
   // 16K to 32K, 8 KV heads of 128 (1.54 GB): 277 -> 255 us; where they fit, and are there from the call before, that would lose
   // (32768 tokens, 8 heads of 128: 28 -> 33 us).  Keys are read 64 bytes of a row at a time, half a cache line, and lose by it
   // at any size.
-  best.past = best.n_blk == 1 && best.vs == 1 && (double)B * H * pages_of(T) * PA_PAGE * D * 4 > HILS_LAST_CACHE;
+  best.past = best.rows == 16 && best.n_blk == 1 && best.vs == 1 && (double)B * H * pages_of(T) * PA_PAGE * D * 4 > HILS_LAST_CACHE;
   return best;
 }
 
