@@ -28,8 +28,8 @@ def rotary_embedding(q, k, positions, inv_freq, interleaved=False, scale=1.0):
     The first ``2 * len(inv_freq)`` features of a head are pairs, features i and i + len(inv_freq), or with ``interleaved``
     2i and 2i + 1; a pair turns by ``positions * inv_freq[i]`` and is multiplied by ``scale``; the other features pass
     through.  ``positions``: int32 or int64, (T,) or (B,T), or an int, the position of the first token.  ``inv_freq``: fp32
-    or fp64 on the GPU (``rotary_frequencies``).  Angles are formed in fp64, so far positions keep their precision; the
-    rotation is fp32 with one rounding.  Differentiable in q and k."""
+    or fp64 on the GPU (``rotary_frequencies``).  Angles and rotation are fp64, so far positions keep their precision; the
+    result is rounded to bf16 by way of fp32: half a step of bf16 and at most 2^-24 more.  Differentiable in q and k."""
     first = 0
     if not isinstance(positions, torch.Tensor):
         first, positions = int(positions), None
@@ -46,7 +46,11 @@ def rotary_frequencies(rotary_dim, base=10000.0, scaling=None, factor=1.0, origi
     * ``"ntk"``         base times factor^(d / (d - 2)): the slowest pair divided by ``factor``, the fastest kept;
     * ``"yarn"``        pairs that turn more than ``high`` (32) times over ``original_length`` kept, fewer than ``low`` (1)
                         divided by ``factor``, between them a ramp in the number of turns; scale 0.1 ln(factor) + 1;
-    * ``"wavelength"``  the same ramp between ``low`` (1) and ``high`` (4) turns, scale 1."""
+    * ``"wavelength"``  the same ramp between ``low`` (1) and ``high`` (4) turns, scale 1.
+
+    The ramp is linear in the number of turns, as the method's formula has it.  A checkpoint trained with a ramp that is
+    linear in the pair's number i, which also goes by the name of yarn, has other frequencies between the two ends: hand
+    ``rotary_embedding`` that model's own ``inv_freq``."""
     rotary_dim = int(rotary_dim)
     if rotary_dim < 2 or rotary_dim % 2:
         raise ValueError(f"rotary_dim must be even and positive, got {rotary_dim}")

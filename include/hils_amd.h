@@ -459,7 +459,7 @@ int hils_norm_rope_pool_bwd_ws(const void* x, const void* norm_weight, const voi
  * (interleaved) 2i and 2i + 1: y1 = scale (x1 cos a - x2 sin a), y2 = scale (x2 cos a + x1 sin a), a = position *
  * inv_freq[i]; the others pass through.  inv_freq (rotary_dim / 2) fp32 or (inv_freq_64) fp64; positions int32 or
  * (positions_64) int64, (T) or (positions_per_batch) (B,T), NULL: first_position + t.  Angles are formed in fp64 turns, the
- * rotation in fp32, rounded once.  sin_sign = -1 is the backward (q, k then hold the gradients of q_out, k_out).
+ * rotation in fp64, rounded to bf16 by way of fp32.  sin_sign = -1 is the backward (q, k then hold the gradients of q_out, k_out).
  * D and rotary_dim multiples of 16, D <= 1024. */
 int hils_rotary(const void* q, const void* k, void* q_out, void* k_out, const void* positions, const void* inv_freq,
                 size_t q_batch_stride, size_t q_token_stride, size_t q_head_stride, size_t k_batch_stride,
