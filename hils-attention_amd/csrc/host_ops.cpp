@@ -11,6 +11,7 @@
 #include <c10/hip/HIPStream.h>
 
 #include <cmath>
+#include <functional>
 #include <string>
 
 #include "../../include/hils_amd.h"
@@ -878,6 +879,23 @@ void written(const Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
+// What an operator without a backward writes in place: a gradient through it would miss the write.
+void may_write(const char* name, std::initializer_list<const Tensor*> ts) {
+  if (wants_grad(ts)) throw std::runtime_error(c10::str(name, " is an inference operator: what it writes to must not require gradients"));
+}
+
+// Its outputs where an input wants a gradient: a backward through them is refused.
+struct RefuseFn : torch::autograd::Function<RefuseFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& a, const Tensor& b, const OptTensor& c, const char* name,
+                               const std::function<variable_list()>& call) {
+    ctx->saved_data["name"] = std::string(name);
+    return call();
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list) {
+    throw std::runtime_error(c10::str(ctx->saved_data["name"].toStringRef(), " is an inference operator: its backward is not supported"));
+  }
+};
+
 // (B, T, heads, D) rows the kernels can read where they are: contiguous features, everything at multiples of 16 bytes
 Tensor strided_rows(const Tensor& t) {
   const bool fits = t.stride(3) == 1 && row_stride(t, 0) % 8 == 0 && row_stride(t, 1) % 8 == 0 && row_stride(t, 2) % 8 == 0 &&
@@ -1029,6 +1047,14 @@ Tensor paged_append(const Tensor& k, const Tensor& v, const Tensor& k_pages, con
                     bool interleaved, double scale) {
   const char* name = "paged_append";
   const Tensor q = opt(q_opt);
+  if (q.defined() && wants_grad({&k, &v, &q})) {
+    const auto call = [&]() -> variable_list {
+      return {paged_append(k, v, k_pages, v_pages, table, seq_len, q_opt, inv_freq, positions, interleaved, scale)};
+    };
+    may_write(name, {&k_pages, &v_pages});
+    return RefuseFn::apply(k, v, maybe(q), name, call)[0];
+  }
+  may_write(name, {&k_pages, &v_pages});
   HOST_ASSERT(k.dim() == 4 && v.sizes() == k.sizes(), name, ": k ", k.sizes(), " and v ", v.sizes(), " must be (B, T, H, D)");
   need_bf16(name, k);
   need_bf16(name, v);
@@ -1069,6 +1095,14 @@ std::tuple<Tensor, Tensor> paged_flex_attn(const Tensor& q, const Tensor& k_page
                                            const py::object& seq_len, int64_t window, const OptTensor& parents_opt,
                                            bool mask_lmk, bool expand, std::optional<double> sm_scale) {
   const char* name = "paged_flex_attn";
+  if (wants_grad({&q, &k_pages, &v_pages})) {
+    const auto call = [&]() -> variable_list {
+      auto [o, lse] = paged_flex_attn(q, k_pages, v_pages, table, seq_len, window, parents_opt, mask_lmk, expand, sm_scale);
+      return {o, lse};
+    };
+    const auto r = RefuseFn::apply(q, k_pages, v_pages, name, call);
+    return {r[0], r[1]};
+  }
   HOST_ASSERT(q.dim() == 4, name, ": q must have four dimensions");
   need_bf16(name, q);
   const int64_t B = q.size(0), T = q.size(1), HQ = q.size(2), D = q.size(3);
@@ -1103,6 +1137,7 @@ std::tuple<Tensor, Tensor> paged_flex_attn(const Tensor& q, const Tensor& k_page
 void paged_accept(const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const py::object& base_len,
                   const Tensor& path) {
   const char* name = "paged_accept";
+  may_write(name, {&k_pages, &v_pages});
   HOST_ASSERT(path.dim() == 2 && path.scalar_type() == at::kInt, name, ": path must be an int32 (B, n) tensor");
   const Pages p = check_pages(name, path, k_pages, v_pages, table, base_len, "base_len", 0);
   const int64_t n = path.size(1);
@@ -1119,6 +1154,7 @@ void paged_accept(const Tensor& k_pages, const Tensor& v_pages, const Tensor& ta
 
 void copy_pages(const std::vector<Tensor>& pools, const Tensor& src, const Tensor& dst) {
   const char* name = "copy_pages";
+  for (const Tensor& t : pools) may_write(name, {&t});
   HOST_ASSERT(!pools.empty() && pools.size() <= 8, name, ": 1 to 8 pools (got ", pools.size(), ")");
   const at::ScalarType dt = src.scalar_type();
   if ((dt != at::kInt && dt != at::kLong) || dst.scalar_type() != dt)

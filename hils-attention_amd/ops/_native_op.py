@@ -61,15 +61,17 @@ def bare(*tensors):
 
 class InferenceOp(torch.autograd.Function):
     """Base class of an operator without a backward: a subclass defines ``label``, ``native(*args)``, ``forward(ctx, *args)``
-    as ``return <subclass>.native(*args)`` and, if it writes to arguments in place, which (``written``).  Its function calls
-    ``native`` itself where that is all that is wanted; ``apply`` is for the other calls: a trace records them as a node,
-    tangents and function transforms are refused, a gradient through the result is refused when it is asked for, and one
-    through what is written, which would miss it, at once."""
+    as ``return <subclass>.native(*args)`` and, if it writes to arguments in place, which (``written``).  A call goes straight
+    to the native operator, which refuses a gradient through its result when it is asked for, and one through what it
+    writes, which would miss the write, at once.  A trace records the call as a node; tangents and function transforms are
+    refused."""
 
     label, written = "", slice(0)
 
     @classmethod
     def apply(cls, *args):
+        if not (_is_tracing() or forward_ad._current_level >= 0 or _in_transform()):
+            return cls.native(*args)
         if torch.is_grad_enabled() and any(t.requires_grad for t in args[cls.written]):
             raise RuntimeError(f"{cls.label} is an inference operator: what it writes to must not require gradients")
         if forward_ad._current_level >= 0 and not _in_transform() and any(

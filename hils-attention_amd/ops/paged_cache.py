@@ -9,7 +9,7 @@ where they are written are refused.
 import torch
 
 from . import _cabi
-from ._native_op import InferenceOp, bare
+from ._native_op import InferenceOp
 
 
 class _PagedAppend(InferenceOp):
@@ -71,10 +71,10 @@ class _CopyPages(InferenceOp):
 def paged_append(k, v, k_pages, v_pages, page_table, seq_len, q=None, inv_freq=None, positions=None, interleaved=False,
                  scale=1.0):
     """Write keys and values (B,T,H,D) of the last T of ``seq_len`` tokens into their pages, in one launch; tokens whose
-    page is not mapped, and sequences shorter than T, are left out.  With ``inv_freq`` the keys, and q (B,T,H_q,D) if given, are rotated on the way as by
-    ``rotary_embedding``, at ``positions`` (B,T) or, without them, at the tokens' slots.  Returns the rotated q or None."""
-    args = (k, v, k_pages, v_pages, page_table, seq_len, q, inv_freq, positions, bool(interleaved), float(scale))
-    return (_PagedAppend.native if bare(k, v, k_pages, v_pages, q) else _PagedAppend.apply)(*args)
+    page is not mapped, and sequences shorter than T, are left out.  With ``inv_freq`` the keys, and q (B,T,H_q,D) if given,
+    are rotated on the way as by ``rotary_embedding``, at ``positions`` (B,T) or, without them, at the tokens' slots.
+    Returns the rotated q or None."""
+    return _PagedAppend.apply(k, v, k_pages, v_pages, page_table, seq_len, q, inv_freq, positions, bool(interleaved), float(scale))
 
 
 def paged_flex_attn(q, k_pages, v_pages, page_table, seq_len, window_size, parents=None, mask_lmk=True,
@@ -88,15 +88,15 @@ def paged_flex_attn(q, k_pages, v_pages, page_table, seq_len, window_size, paren
     and those that follow them, see nothing (padding).  Without ``parents`` the tokens are a chain.  T <= 256 for a tree.
     Returns o (B,T,H_q,D) bf16 and lse (B,T,H_q) fp32, natural log; rows that see nothing: 0 and -inf.  The same call gives
     the same bits; a sequence's last bits may depend on how many others, and how long ones, are in the batch."""
-    args = (q, k_pages, v_pages, page_table, seq_len, int(window_size), parents, bool(mask_lmk), bool(expand_to_chunk), sm_scale)
-    return (_PagedFlexAttn.native if bare(q, k_pages, v_pages) else _PagedFlexAttn.apply)(*args)
+    return _PagedFlexAttn.apply(q, k_pages, v_pages, page_table, seq_len, int(window_size), parents, bool(mask_lmk),
+                                bool(expand_to_chunk), sm_scale)
 
 
 def paged_accept(k_pages, v_pages, page_table, base_len, path):
     """Move accepted drafts to the front: keys and values at slots ``base_len + path[b][i]`` go to ``base_len + i``.
     ``path`` int32 (B,n) on the GPU, growing strictly; the first entry that does not (-1, say) ends it.  The pages from slot
     ``base_len`` on must be the sequence's own."""
-    (_PagedAccept.native if bare(k_pages, v_pages) else _PagedAccept.apply)(k_pages, v_pages, page_table, base_len, path)
+    _PagedAccept.apply(k_pages, v_pages, page_table, base_len, path)
 
 
 def copy_pages(pools, src, dst):
@@ -116,4 +116,4 @@ def copy_pages(pools, src, dst):
             raise ValueError("copy_pages: a page that is written is in another pair too")
         dev = pools[0].device if pools else None
         src, dst = (torch.tensor(x, dtype=torch.int64, device=dev) for x in (src, dst))
-    (_CopyPages.native if bare(*pools) else _CopyPages.apply)(src, dst, *pools)
+    _CopyPages.apply(src, dst, *pools)

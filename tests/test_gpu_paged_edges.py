@@ -162,3 +162,32 @@ def test_update_keeps_gradients_of_the_chunk_keys(pkg, dev):
         c.fork([0, 0])
         c.update(k[:, :1], k[:, :1])
     assert c.seq_len == 132
+
+
+def test_a_backward_through_an_inference_operator_is_refused(pkg, dev):
+    note("inputs that want gradients")
+    gen = torch.Generator().manual_seed(7)
+    kp, vp, table = ref.cache(gen, 1, 2, 2, 64, dev)
+    k, q = (torch.randn(1, 2, h, 64, generator=gen).bfloat16().to(dev) for h in (2, 4))
+    inv, _ = pkg.rotary_frequencies(64, device=dev)
+    append = lambda k, v, q: pkg.paged_append(k, v, kp, vp, table, 10, q=q, inv_freq=inv)
+    want = append(k, k, q)
+    for i in range(3):
+        args = [k, k, q]
+        args[i] = args[i].clone().requires_grad_()
+        out = append(*args)
+        assert torch.equal(out, want)
+        with pytest.raises(RuntimeError, match="paged_append is an inference operator"):
+            out.float().sum().backward()
+        with torch.no_grad():
+            assert not append(*args).requires_grad
+    assert pkg.paged_append(k.clone().requires_grad_(), k, kp, vp, table, 10) is None
+    want = pkg.paged_flex_attn(q, kp, vp, table, 10, 64)
+    for i in range(3):
+        args = [q, kp, vp]
+        args[i] = args[i].clone().requires_grad_()
+        o, lse = pkg.paged_flex_attn(*args, table, 10, 64)
+        assert torch.equal(o, want[0]) and torch.equal(lse, want[1])
+        for x in (o, lse):
+            with pytest.raises(RuntimeError, match="paged_flex_attn is an inference operator"):
+                x.float().sum().backward()

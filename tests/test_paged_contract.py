@@ -179,20 +179,15 @@ def test_tangents_and_transforms_are_refused(pkg, monkeypatch):
             call(*args)  # (no tangent: nothing is lost)
 
 
-def test_pages_that_require_gradients_are_not_written(pkg, monkeypatch):
-    _stand_in(monkeypatch)
+def test_pages_that_require_gradients_are_not_written(pkg):
+    """(refused by the native operators, before they look where the tensors are)"""
     for name, call, written in _calls(pkg):
         for i in written:
             args = _tensors(1)
             args[i].requires_grad_()
-            was = [x.detach().clone() for x in args]
             with pytest.raises(RuntimeError, match=f"{name} .* must not require gradients"):
                 call(*args)
-            assert all(torch.equal(x, y) for x, y in zip(args, was))
-            with torch.no_grad():
+            with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU path"):
                 call(*args)
-        if not written:
-            args = _tensors(1)
-            out = call(*[x.requires_grad_() for x in args])
-            with pytest.raises(RuntimeError, match=f"{name} is an inference operator"):
-                out.float().sum().backward()
+            with forward_ad.dual_level(), pytest.raises(RuntimeError, match=f"{name} .* must not require gradients"):
+                call(*args)
