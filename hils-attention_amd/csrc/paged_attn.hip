@@ -12,12 +12,16 @@
 //   paged_attn_rows   16 or 32 rows a workgroup, its wavefronts share the keys (bound by the memory system),
 //   paged_attn_tiles  64, 128 or 256 rows a workgroup, 32 a wavefront, pages staged in LDS (bound by the matrix and vector units).
 // A long range of keys is split over workgroups; paged_attn_join adds their shares up, in a fixed order.
-// Scores, maxima, sums and outputs are fp32; probabilities are rounded to bf16 for the second product (half a step of
-// 2^-9 each, of random sign, about the size of the output's own rounding), their sum is taken before the rounding.
+// Scores, maxima, sums and outputs are fp32; probabilities are rounded to bf16 for the second product, their sum is taken before
+// the rounding.  Each is off by up to 2^-8 of itself, of random sign, which adds as much to an output's error as its own rounding:
+// 2.0e-3 to 2.4e-3 of the output's norm against 64 bits, 1.6e-3 where the output alone is rounded.  (Two products with a
+// probability's leading and next bits would keep the latter, for half as many matrix instructions again.)
 //
-// Values at slots that a row does not see meet a probability of exactly 0, which an infinity or a NaN there (a stale slot
-// behind the last token, a rejected draft) would turn into a NaN.  A row whose result is no finite number is therefore
-// computed once more, token by token over the slots that it sees alone (paged_redo_row): the common call pays a comparison.
+// Values at slots that a row does not see meet a probability of exactly 0, which an infinity or a NaN there would turn into a
+// NaN.  Behind the last token, where a page holds what its last user left, values are read as zeros.  Elsewhere (a token before
+// the window, a landmark, another branch's draft) a row whose result is no finite number is computed once more, token by token
+// over the slots that it sees alone (paged_redo_row): the common call pays a comparison, a call all of whose rows take that
+// way 12 times its time (one token) to 160 times (trees: 92 us become 15 ms).
 #include <string.h>
 
 #include "common.h"
@@ -337,7 +341,7 @@ paged_attn_rows(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, cons
   const int32_t* table = dm.table + (long)b * dm.max_pages;
   const int t0 = hils_udiv(r0, dm.G, dm.g_magic);
 
-  const int u0 = sp.p0 * 2, u1 = sp.p1 * 2;
+  const int u0 = sp.p0 * 2, u1 = sp.p1 * 2, len = __builtin_amdgcn_readfirstlane(at.len);
   // page of the units that this wavefront takes: lane i holds that of its i-th one
   int pages_of = -1;
   auto ask_pages = [&](int first) __attribute__((always_inline)) {
@@ -395,6 +399,11 @@ paged_attn_rows(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, cons
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int i = 0; i < VI; ++i) *(pa_u4*)(w_addr + i * TPI * VP) = vd[i];
+    if (u * 32 + 32 > len) {  // (the same for the whole wavefront) values behind the last token: zeros
+#pragma unroll
+      for (int i = 0; i < VI; ++i)
+        if (u * 32 + lane / VL + i * TPI >= len) *(pa_u4*)(w_addr + i * TPI * VP) = pa_u4{0, 0, 0, 0};
+    }
     __builtin_amdgcn_wave_barrier();
     f32x4_t S[NR][2];
 #pragma unroll
@@ -883,6 +892,17 @@ paged_attn_tiles(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, con
 #undef PA_HALF
 #undef PA_PAIR
   };
+  // Values behind the last token: zeros, as soon as this wavefront's loads of them have landed (and before the barrier behind
+  // which the others read them).
+  const int rows_in = at.len - (p0 + n - 1) * PA_PAGE;  // of the last page
+  auto clear_behind = [&](int x) __attribute__((always_inline)) {
+    if (x < n - 1 || rows_in >= PA_PAGE) return;
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int piece = (wave * NP + i) * 64 + lane;
+      if (piece / SEG >= rows_in) *(uint4*)(pa_dyn + (NB + ((x & 3) ^ (x >> 1 & 1))) * PAGE + piece * 16) = make_uint4(0, 0, 0, 0);
+    }
+  };
   auto turn_k = [&](int x) __attribute__((always_inline)) {  // the bit in which the buffers of pages x and x + 1 differ
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) k_off[ks] ^= x & 1 ? 2 * PAGE : PAGE;
@@ -902,6 +922,7 @@ paged_attn_tiles(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, con
     (void)settle(sa, pa, highest(sa));
     for (int x = 0; x < n; ++x) {
       lz_landed<4 * NP>();  // keys of x + 1, values of x
+      clear_behind(x);
       lds_barrier();        // ... of all wavefronts; keys of x and values of x - 1 have been read
       const unsigned long long v_from = v_pool + place;
       place = page_place(x + 4);
@@ -924,6 +945,7 @@ paged_attn_tiles(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, con
     fetch(k_pool + place_k, k_buffer(4));
     auto one = [&](int x, f32x16_t& s1, f32x16_t& s2, pa_u4 (&p1)[2], pa_u4 (&p2)[2]) __attribute__((always_inline)) {
       lz_landed<4 * NP>();  // keys of x + 2, values of x
+      clear_behind(x);
       lds_barrier();        // ... of all wavefronts; keys of x + 1 and values of x - 1 have been read
       const unsigned long long v_from = v_pool + place;
       place = place_k;
