@@ -18,7 +18,8 @@
 // probability's leading and next bits would keep the latter, for half as many matrix instructions again.)
 //
 // Values at slots that a row does not see meet a probability of exactly 0, which an infinity or a NaN there would turn into a
-// NaN.  Behind the last token, where a page holds what its last user left, values are read as zeros.  Elsewhere (a token before
+// NaN.  Behind the last token, where a page holds what its last user left, and in place of a page that is not mapped values are
+// read as zeros.  Elsewhere (a token before
 // the window, a landmark, another branch's draft) a row whose result is no finite number is computed once more, token by token
 // over the slots that it sees alone (paged_redo_row): the common call pays a comparison, a call all of whose rows take that
 // way 12 times its time (one token) to 160 times (trees: 92 us become 15 ms).
@@ -892,15 +893,16 @@ paged_attn_tiles(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, con
 #undef PA_HALF
 #undef PA_PAIR
   };
-  // Values behind the last token: zeros, as soon as this wavefront's loads of them have landed (and before the barrier behind
-  // which the others read them).
+  // Values behind the last token, and of a page that is not mapped: zeros, as soon as this wavefront's loads of them have
+  // landed (and before the barrier behind which the others read them).
   const int rows_in = at.len - (p0 + n - 1) * PA_PAGE;  // of the last page
-  auto clear_behind = [&](int x) __attribute__((always_inline)) {
-    if (x < n - 1 || rows_in >= PA_PAGE) return;
+  auto clear_stale = [&](int x, int back) __attribute__((always_inline)) {  // back: fetches of keys since page x
+    const int rows = !(known >> back & 1) ? 0 : x < n - 1 ? PA_PAGE : rows_in;
+    if (rows >= PA_PAGE) return;
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
       const int piece = (wave * NP + i) * 64 + lane;
-      if (piece / SEG >= rows_in) *(uint4*)(pa_dyn + (NB + ((x & 3) ^ (x >> 1 & 1))) * PAGE + piece * 16) = make_uint4(0, 0, 0, 0);
+      if (piece / SEG >= rows) *(uint4*)(pa_dyn + (NB + ((x & 3) ^ (x >> 1 & 1))) * PAGE + piece * 16) = make_uint4(0, 0, 0, 0);
     }
   };
   auto turn_k = [&](int x) __attribute__((always_inline)) {  // the bit in which the buffers of pages x and x + 1 differ
@@ -922,7 +924,7 @@ paged_attn_tiles(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, con
     (void)settle(sa, pa, highest(sa));
     for (int x = 0; x < n; ++x) {
       lz_landed<4 * NP>();  // keys of x + 1, values of x
-      clear_behind(x);
+      clear_stale(x, 3);
       lds_barrier();        // ... of all wavefronts; keys of x and values of x - 1 have been read
       const unsigned long long v_from = v_pool + place;
       place = page_place(x + 4);
@@ -945,7 +947,7 @@ paged_attn_tiles(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, con
     fetch(k_pool + place_k, k_buffer(4));
     auto one = [&](int x, f32x16_t& s1, f32x16_t& s2, pa_u4 (&p1)[2], pa_u4 (&p2)[2]) __attribute__((always_inline)) {
       lz_landed<4 * NP>();  // keys of x + 2, values of x
-      clear_behind(x);
+      clear_stale(x, 4);
       lds_barrier();        // ... of all wavefronts; keys of x + 1 and values of x - 1 have been read
       const unsigned long long v_from = v_pool + place;
       place = place_k;

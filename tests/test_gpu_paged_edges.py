@@ -228,3 +228,27 @@ def test_what_lies_behind_the_last_token_costs_nothing(pkg, dev, heads, B, T, le
     print(f"    {clean:.1f} us, {spoilt:.1f} with stale numbers", flush=True)
     assert all(torch.equal(x, y) for x, y in zip(want, got))
     assert spoilt <= 2 * clean + 20
+
+
+@pytest.mark.parametrize("heads,T,window", [((32, 8, 128), 63, 512), ((32, 4, 128), 64, 1 << 20), ((16, 4, 64), 64, 1 << 20),
+                                            ((32, 8, 128), 1, 1 << 20)])
+def test_what_lies_in_the_pools_first_page_costs_nothing(pkg, dev, heads, T, window):
+    """A sequence with pages that are not mapped, and a first page of the pools that is nobody's and holds no numbers."""
+    note(f"pages that are not mapped beside a stale first page, heads {heads}, {T} tokens")
+    HQ, H, D = heads
+    B, length = 3, 4093
+    gen = torch.Generator().manual_seed(T)
+    k, v, table = ref.cache(gen, B, 64, H, D, dev)
+    table[table == 0] = k.shape[0] - 1 if not (table == k.shape[0] - 1).any() else -1
+    table[0, 60], table[1, 58:61], table[2, :62] = -1, 10 ** 6, -1
+    q = torch.randn(B, T, HQ, D, generator=gen).bfloat16().to(dev)
+    parents = torch.tensor(ref.tree(gen, T), dtype=torch.int32, device=dev) if T > 1 else None
+    call = lambda: pkg.paged_flex_attn(q, k, v, table, length, window, parents=parents)
+    k[0] = v[0] = 0
+    want, clean = call(), _shortest(call)
+    k[0] = v[0] = float("nan")
+    got, spoilt = call(), _shortest(call)
+    print(f"    {clean:.1f} us, {spoilt:.1f} with stale numbers", flush=True)
+    assert all(torch.equal(x, y) for x, y in zip(want, got))
+    assert spoilt <= 2 * clean + 20
+    ref.check_attention(got, ref.attend(q, k, v, table, length, window, None if parents is None else parents.cpu()))
