@@ -590,9 +590,12 @@ paged_attn_rows(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, cons
 // wavefront overlap, those of two that run in step hardly do).  The exponentials' reference point follows a row's maximum
 // only when a score is more than 2^6 above it: the others need no reduction over lanes and no rescaling, and probabilities
 // of up to 2^6 enter sum and output alike.
-// Bound by latencies where a window has ten pages (17.4 us for trees of 63 tokens for 8 sequences, 8 KV heads of 128: 7.6 in
-// the steps), else by the vector and matrix units together: 1.6 us a page of 256 rows, 0.85 of it matrix products; trees of 64
-// tokens for 4 sequences of 8K to 16K, 4 KV heads of 128, everything seen: 72 us with the join (51 GFLOP).
+// Bound by latencies where a window has ten pages (18 us for trees of 63 tokens for 8 sequences, 8 KV heads of 128: 7.6 in the
+// steps), else by the vector and matrix units together.  A page of 256 rows takes 1.6 us where 32 workgroups have the chip to
+// themselves, 0.85 of it matrix products, and 2.25 with one on every compute unit (four trees of 64 tokens, 4 KV heads of 128,
+// everything seen: 89 us for 32 pages a workgroup, 312 for 128: 0.95 PFLOP/s in the steps, 1.41 in a large product).
+// Sequences of 8K to 16K: 72 to 78 us with the join (51 GFLOP): 25 to 28 pages of the longest share, 7 us of start and end,
+// the join's 10.
 // The buffers come first: their places are then plain offsets, and a buffer's number is two bits of them.
 template <int D, int NW, int KW, bool TREE>
 static constexpr size_t paged_tiles_smem() {
@@ -1029,7 +1032,7 @@ paged_attn_tiles(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, con
 
 // ---- shares of a range added up ------------------------------------------------------------------
 // A wavefront a row: lane i weighs share i (there are up to 64), then groups of D / 4 lanes take every GR-th share, four loads
-// under way, and add up across the groups.  Bound by HBM or the launch: 32768 rows of 8 shares (34 MB) in 7.5 to 10 us.
+// under way, and add up across the groups.  Bound by HBM or the launch: 8192 rows of 8 shares (34 MB) in 7.5 to 10 us, 512 in 5.
 template <int D>
 __global__ void __launch_bounds__(256) paged_attn_join(PagedDims dm, PagedOut out) {
   constexpr int LPR = D / 4, GR = 64 / LPR;  // lanes per row of features, groups
@@ -1102,6 +1105,10 @@ struct PagedPlan {
 // within 2 % of the best measured one on average and within 17 % in the worst of 187 calls; fixed
 // thresholds on rows and pages were 15 % off on average and lost up to 1.7 times (1 token, 8 KV heads of 128, 4096 tokens: 8
 // shares 12.9 us, 32 shares 8.5; 16 tokens, 2 KV heads of 64, window 512: 32 rows a workgroup 10.1, 16 rows 7.5).
+// What this does not cover: page tables much wider than the sequences.  All pages that the table and the window allow count,
+// and short sequences in a long table are cut into shares, and given row blocks, that are meant for more keys: 512 tokens, 32 / 8
+// heads of 128, in tables of 8 and of 2048 pages: one token of one sequence 7.3 and 8.8 us, of 16 sequences 7.8 and 24, four
+// trees of 64 (4 KV heads) 15 and 29.  And `page` of the 256-row variant is that of a chip with few workgroups.
 struct PagedCost {
   int rows, vs, nw, kw;
   float fixed, start, page, beside;
@@ -1154,11 +1161,12 @@ static PagedPlan paged_choose(int B, int T, int HQ, int H, int D, int window, in
       best.n_split = n_split;
     }
   }
-  // One row block of 16 reads a key and a value once.  Where all of them do not fit the last cache, values go past it: 16 sequences of
-  // 16K to 32K, 8 KV heads of 128 (1.54 GB): 277 -> 255 us; where they fit, and are there from the call before, that would lose
+  // One row block of 16 reads a key and a value once.  Where all of them do not fit the last cache, values go past it: 16 sequences
+  // of 16K to 32K, 8 KV heads of 128 (1.54 GB): 277 -> 255 us; where they fit, and are there from the call before, that would lose
   // (32768 tokens, 8 heads of 128: 28 -> 33 us).  Keys are read 64 bytes of a row at a time, half a cache line, and lose by it
   // at any size.
-  best.past = best.rows == 16 && best.n_blk == 1 && best.vs == 1 && (double)B * H * pages_of(T) * PA_PAGE * D * 4 > HILS_LAST_CACHE;
+  best.past = best.rows == 16 && best.n_blk == 1 && best.vs == 1 &&
+              (double)B * H * pages_of(T) * PA_PAGE * D * 4 > HILS_LAST_CACHE;
   return best;
 }
 

@@ -146,7 +146,9 @@ rotary_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, const 
     const double turns = p * (w * 0.15915494309189533577);  // 1 / (2 pi)
     double sn, cs;
     sincospi(2.0 * (turns - rint(turns)), &sn, &cs);
-    const int at = i ^ (i >> 4 & 2);  // (eight units in step read angles 64 bytes apart: of two that share banks one reads ahead)
+    // (eight units in step read angles 64 bytes apart; of two that are 256 bytes apart one reads its second pair first: 136.7 -> 134.4
+    // us for the prompts' append.  Half of the LDS unit's busy cycles, a quarter of the kernel's, still count as bank conflicts.)
+    const int at = i ^ (i >> 4 & 2);
     cos_s[at] = cs * dm.scale;
     sin_s[at] = sn * dm.scale * dm.sign;
   }

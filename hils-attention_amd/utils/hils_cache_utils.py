@@ -617,8 +617,9 @@ class HiLSPagedLayer:
                                  prior_pages=self.prior_pages if self.has_prior else None)
 
     def _drafts_attend(self, q, lse_swa, topk, window_size, sm_scale, dense_keys):
-        """A token at position p selects among the chunks before floor((p - window + 1) / 64): tokens with the same limit
-        go through one call, up to 64 of them at positions whose limit with a window of 1 is that one."""
+        """A token at position p selects among the chunks before floor((p - window + 1) / 64).  For every such limit that
+        occurs all tokens go through a call, up to 64 at a time, at positions whose limit with a window of 1 is that one, and
+        those whose limit it is take its results: a tree across a chunk's border costs twice."""
         S, T = self.S, self.drafted
         assert q.shape[1] == T, f"{T} tokens are on trial, got {q.shape[1]} queries"
         back = window_size - 1 if window_size > 0 else 0
