@@ -1081,7 +1081,8 @@ Tensor paged_append(const Tensor& k, const Tensor& v, const Tensor& k_pages, con
   const Tensor ks = strided_rows(k), vs = strided_rows(v), qs = HQ ? strided_rows(q) : Tensor();
   const Tensor pos = c.positions.defined() ? c.positions.contiguous() : Tensor();
   HILS_CALL(hils_paged_append, cptr(qs), cptr(ks), cptr(vs), HQ ? mptr(qo) : nullptr, mptr(k_pages), mptr(v_pages), iptr(table),
-            iptr(p.lengths), cptr(pos), cptr(c.inv_freq), ROW_STRIDES(qs), ROW_STRIDES(ks), ROW_STRIDES(vs), i32(B), i32(T), i32(HQ), i32(H), i32(D),
+            iptr(p.lengths), cptr(pos), cptr(c.inv_freq), ROW_STRIDES(qs), ROW_STRIDES(ks), ROW_STRIDES(vs), i32(B), i32(T),
+            i32(HQ), i32(H), i32(D),
             i32(c.inv_freq.defined() ? 2 * c.inv_freq.numel() : 0), (int)interleaved,
             (int)(pos.defined() && pos.scalar_type() == at::kLong),
             (int)(c.inv_freq.defined() && c.inv_freq.scalar_type() == at::kDouble), i32(p.max_pages), i32(p.pages),

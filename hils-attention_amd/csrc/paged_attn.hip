@@ -12,17 +12,16 @@
 //   paged_attn_rows   16 or 32 rows a workgroup, its wavefronts share the keys (bound by the memory system),
 //   paged_attn_tiles  64, 128 or 256 rows a workgroup, 32 a wavefront, pages staged in LDS (bound by the matrix and vector units).
 // A long range of keys is split over workgroups; paged_attn_join adds their shares up, in a fixed order.
-// Scores, maxima, sums and outputs are fp32; probabilities are rounded to bf16 for the second product, their sum is taken before
-// the rounding.  Each is off by up to 2^-8 of itself, of random sign, which adds as much to an output's error as its own rounding:
-// 2.0e-3 to 2.4e-3 of the output's norm against 64 bits, 1.6e-3 where the output alone is rounded.  (Two products with a
+// Scores, maxima, sums and outputs are fp32; probabilities are rounded to bf16 for the second product, their sum is taken
+// before the rounding.  Each is off by up to 2^-8 of itself, of random sign, which adds as much to an output's error as its own
+// rounding: 1.9e-3 to 2.4e-3 of the output's norm against 64 bits, 1.6e-3 where the output alone is rounded.  (Two products with a
 // probability's leading and next bits would keep the latter, for half as many matrix instructions again.)
 //
 // Values at slots that a row does not see meet a probability of exactly 0, which an infinity or a NaN there would turn into a
-// NaN.  Behind the last token, where a page holds what its last user left, and in place of a page that is not mapped values are
-// read as zeros.  Elsewhere (a token before
-// the window, a landmark, another branch's draft) a row whose result is no finite number is computed once more, token by token
-// over the slots that it sees alone (paged_redo_row): the common call pays a comparison, a call all of whose rows take that
-// way 12 times its time (one token) to 160 times (trees: 92 us become 15 ms).
+// NaN.  Behind the last token, where a page holds what its last user left, and in place of a page that is not mapped values
+// are read as zeros.  Elsewhere (a token before the window, a landmark, another branch's draft) a row whose result is no finite
+// number is computed once more, token by token over the slots that it sees alone (paged_redo_row): the common call pays a
+// comparison, a call all of whose rows take that way 12 times its time (one token) to 190 times (trees: 88 us become 17 ms).
 #include <string.h>
 
 #include "common.h"

@@ -239,10 +239,12 @@ class HiLSPagedLayer:
     free list, so the page order of a sequence is arbitrary.
 
     Sequences may share pages after ``fork``: a page counts its users, returns to the free list when the last one lets go
-    of it, and is copied before a sequence writes on a page that others use too.  Keys and values that require gradients
-    get them through the pages (``gather_contiguous``, the chunk keys); the attention on the pages itself has no backward.  ``draft`` appends tokens on trial, in a
+    of it, and is copied before a sequence writes on a page that others use too.  ``draft`` appends tokens on trial, in a
     chain or a tree; ``local_attend`` and ``hils_attend`` then are for them, and ``accept`` keeps a path of the tree and
-    drops the rest.  ``truncate`` and ``free`` give tokens up, ``compact`` gathers the pages in use at the front."""
+    drops the rest.  ``truncate`` and ``free`` give tokens up, ``compact`` gathers the pages in use at the front.
+
+    Keys and values that require gradients get them through the pages (``gather_contiguous``, the chunk keys); the attention
+    on the pages itself has no backward."""
 
     def __init__(self, num_pages, batch, max_pages_per_seq, num_kv_heads, head_dim, device,
                  num_q_heads=None, chunk_pooling=True, page_order=None, dtype=torch.bfloat16):
